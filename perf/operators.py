@@ -83,7 +83,7 @@ def draw(rng):
     D = rng.choice([64, 128, 128, 80])
     Hkv = rng.choice([1, 2, 4, 8])
     H = Hkv * rng.choice([1, 2, 4, 7])
-    block = rng.choice([16, 32, 32, 64, 128])
+    block = rng.choice([32, 32, 64, 128])
     cache = rng.choice(["int8", "int8", "e4m3"])
     if kind == "rope":
         mixed = rng.random() < 0.5
