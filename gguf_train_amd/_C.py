@@ -21,6 +21,7 @@ LIB_PATH = _PKG_DIR / "libgt_attn.so"
 # dtype / device codes (csrc/gguf_train.h:22-44)
 GT_F32, GT_F16, GT_BF16, GT_F64 = 0, 1, 2, 3
 GT_I8, GT_U8, GT_I16, GT_I32, GT_I64, GT_BOOL = 4, 5, 6, 7, 8, 9
+GT_F8E4M3 = 12  # codes of a block cache (no counterpart in the reference)
 GT_Q_BASE = 100
 GT_Q8_0 = GT_Q_BASE + 8
 GT_DEV_CPU, GT_DEV_CUDA = 0, 1
@@ -183,6 +184,11 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
                                             c_int, c_float, c_float]
     lib.gt_flash_attention_rope.restype = c_void_p
 
+    # several axes (no counterpart in the reference ABI)
+    for fn in (lib.gt_rope_axes, lib.gt_rope_axes_backward):
+        fn.argtypes = [c_void_p, c_void_p, c_int, POINTER(c_int), c_int, c_int, c_int, c_double, c_double]
+        fn.restype = c_void_p
+
     # Q8_0 (csrc/gguf_train.h:381-382)
     lib.gt_quantize.argtypes = [c_void_p, c_int]
     lib.gt_quantize.restype = c_void_p
@@ -211,6 +217,21 @@ def _configure(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.gt_kv_cache_append_rope.restype = c_int
     lib.gt_kv_cache_attention.argtypes = [c_void_p, c_void_p, c_float, c_int]
     lib.gt_kv_cache_attention.restype = c_void_p
+    lib.gt_kv_cache_create_blocks.argtypes = [c_int64, c_int64, c_int64, c_int64, c_int, c_int, c_int]
+    lib.gt_kv_cache_create_blocks.restype = c_void_p
+    lib.gt_kv_cache_read.argtypes = [c_void_p, c_int, p_vp, p_vp]
+    lib.gt_kv_cache_read.restype = c_int
+    lib.gt_kv_cache_append_rope_axes.argtypes = [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, POINTER(c_int),
+                                                 c_int, c_int, c_int, c_double, c_double]
+    lib.gt_kv_cache_append_rope_axes.restype = c_int
+    lib.gt_kv_cache_attention_accumulate.argtypes = [c_void_p, c_void_p, c_float, c_int, c_float]
+    lib.gt_kv_cache_attention_accumulate.restype = c_void_p
+    lib.gt_kv_cache_weights.argtypes = [c_void_p]
+    lib.gt_kv_cache_weights.restype = c_void_p
+    lib.gt_kv_cache_evict.argtypes = [c_void_p, c_int64, c_int64, c_void_p, p_vp]
+    lib.gt_kv_cache_evict.restype = c_int
+    lib.gt_kv_cache_position.argtypes = [c_void_p, c_int64]
+    lib.gt_kv_cache_position.restype = c_int64
 
     # GGUF read side (csrc/gguf_train.h:363-379; gguf_train/_C.py:527-560)
     lib.gt_gguf_open.argtypes = [c_char_p]

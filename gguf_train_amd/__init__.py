@@ -8,10 +8,10 @@ MultiheadAttention with the reference's signatures, and the GGUF Q8_0 codec.
 
 from . import _C
 from ._bridge import QuantizedTensor
-from ._functions import FlashAttentionDropoutFn, FlashAttentionFn, RoPEFn
+from ._functions import FlashAttentionDropoutFn, FlashAttentionFn, RoPEAxesFn, RoPEFn
 from ._ops import (attention_dropout_mask, attention_weights_dropout, dequantize, flash_attention,
                    flash_attention_backward, flash_attention_dropout, flash_attention_dropout_backward,
-                   flash_attention_lse, flash_attention_rope, flash_attention_train, quantize, rope)
+                   flash_attention_lse, flash_attention_rope, flash_attention_train, quantize, rope, rope_axes)
 from . import nn
 from .kv_cache import KVCache
 
@@ -21,7 +21,9 @@ __all__ = [
     "FlashAttentionFn",
     "FlashAttentionDropoutFn",
     "RoPEFn",
+    "RoPEAxesFn",
     "rope",
+    "rope_axes",
     "flash_attention",
     "flash_attention_lse",
     "flash_attention_train",

@@ -4,6 +4,8 @@
 pos, n_dims, mode, n_ctx_orig, freq_base, freq_scale) saves the positions and calls the native
 gt_rope; the backward calls gt_rope_backward (the inverse rotation) and returns (gx, None x 6).
 
+`RoPEAxesFn` is the same for positions on several axes (gt_rope_axes), which the reference refuses.
+
 `FlashAttentionFn` keeps the reference's signature and behaviour
 (gguf_train/_functions.py:1922-1965): forward(ctx, q, k, v, mask, scale, is_causal) saves
 its inputs, sets ctx.scale (1/sqrt(D) when None) and ctx.is_causal, and calls the native
@@ -48,6 +50,25 @@ class RoPEFn(torch.autograd.Function):
         (pos,) = ctx.saved_tensors
         gx = _ops.rope(grad_out, pos, *ctx.args, backward=True)
         return (gx, None, None, None, None, None, None)
+
+
+class RoPEAxesFn(torch.autograd.Function):
+    """RoPE with positions on several axes; the backward is the inverse rotation, itself differentiable."""
+
+    @staticmethod
+    def forward(ctx, x, pos, sections, n_dims, mode, interleaved, freq_base, freq_scale, inverse=False):
+        ctx.args = (tuple(sections), int(n_dims), int(mode), bool(interleaved), float(freq_base), float(freq_scale))
+        ctx.inverse = bool(inverse)
+        ctx.save_for_backward(pos)
+        return _ops.rope_axes(x, pos, *ctx.args, backward=ctx.inverse)
+
+    @staticmethod
+    def backward(ctx, grad_out):
+        if grad_out is None:
+            return (None,) * 9
+        (pos,) = ctx.saved_tensors
+        gx = RoPEAxesFn.apply(grad_out, pos, *ctx.args, not ctx.inverse)
+        return (gx, None, None, None, None, None, None, None, None)
 
 
 class FlashAttentionFn(torch.autograd.Function):

@@ -180,6 +180,23 @@ def rope(x, pos, n_dims: int, mode: int = 0, n_ctx_orig: int = 0, freq_base: flo
     return adopt(ptr, "rope")
 
 
+def section_list(sections):
+    """(count, C array) of the pairs per axis; the entry points check the numbers."""
+    vals = [int(n) for n in sections]
+    return len(vals), (ctypes.c_int * max(len(vals), 1))(*vals)
+
+
+def rope_axes(x, pos, sections, n_dims: int, mode: int = 2, interleaved: bool = False, freq_base: float = 10000.0,
+              freq_scale: float = 1.0, backward: bool = False) -> torch.Tensor:
+    """gt_rope_axes / gt_rope_axes_backward: RoPE of tokens with positions on several axes."""
+    bind_stream(_device_of(x))
+    hx, hp = borrow(x), borrow(pos)
+    n, sec = section_list(sections)
+    fn = _C.lib.gt_rope_axes_backward if backward else _C.lib.gt_rope_axes
+    ptr = fn(hx.ptr, hp.ptr, n, sec, 1 if interleaved else 0, int(n_dims), int(mode), float(freq_base), float(freq_scale))
+    return adopt(ptr, "rope_axes")
+
+
 def flash_attention_rope(q, k, v, pos, mask=None, scale: float = 0.0, is_causal: bool = False, n_dims=None,
                          mode: int = 0, freq_base: float = 10000.0, freq_scale: float = 1.0) -> torch.Tensor:
     """gt_flash_attention_rope: attention of rope(q, pos) and rope(k, pos), the query rotation fused

@@ -1,0 +1,271 @@
+// The attention weight that a cache's tokens receive: for a call's queries over the cache (B, Hkv, cap, D),
+//   a[b, g, t] <- f a[b, g, t] + sum over the group's heads h and the rows l of exp(scale q_hl . k_t - lse_hl),
+// the column sums of the softmax that the attention of the same call has just formed, from its log-sum-exp.
+//
+// Bound: at few rows the keys, read once more (half the attention's bytes, much of it from the caches); at many
+// the products.  A wavefront owns 16 TW keys, whose operands stay in registers while it walks the rows in
+// columns of 16 (row r = head * L + token): S^T = K.Q^T on v_mfma_f32_16x16x32_f16, exp, a sum per lane, and at
+// the end a sum over the 16 lanes of a key's row.  One writer per sum, so no atomics and the same bits each time;
+// where few wavefronts meet many rows the columns are split, and a second launch adds the splits in order.
+//
+// Operands as attn_kv_blocks.h has them: codes are exact in float16; other rows of keys (bfloat16, float32,
+// Q8_0 values, a block cache's tail) are divided by their own power of two and enter as float16 hi, or as
+// hi + lo where they hold more bits than float16 (float32, Q8_0); float32 queries as hi + lo.
+
+#include "attn_kv_blocks.h"
+
+#include <cmath>
+
+namespace {
+
+using namespace gtkvb;
+
+enum Source { kInt8, kE4m3, kF16, kBf16, kF32, kQ8 };
+
+struct Args {
+    const void *q;
+    int64_t q_sb, q_sh, q_sl;
+    const char *k;  // rows (B, Hkv, cap); the codes of a block cache
+    int64_t row_bytes, cap;
+    const float *ks, *kt;  // a block cache's scales and tail
+    int N;
+    int64_t units;
+    const float *lse;
+    const int32_t *len;
+    float *sums;   // (B, Hkv, cap)
+    float *parts;  // (splits, B, Hkv, cap), or null: one split writes sums
+    float keep;
+    float scale;
+    int causal, q_vec;
+    int H, Hkv, L, D;
+    int col_tiles, span;  // columns of 16 rows in all, and per split
+};
+
+__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kF32>) { return ((const float *)row)[d]; }
+__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kF16>) { return (float)((const _Float16 *)row)[d]; }
+__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kBf16>) { return (float)((const __bf16 *)row)[d]; }
+__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kQ8>) {
+    const uint8_t *blk = (const uint8_t *)row + (d >> 5) * 34;
+    return (float)*(const _Float16 *)blk * (float)*(const int8_t *)(blk + 2 + (d & 31));
+}
+
+// The A operands of key `t` (this lane's, of 16; zeros when it is not there) and its scale; lanes g hold dims
+// 16 (4i + g) .. +15.
+template <int KIND, int NI>
+__device__ inline float key_operands(const char *row, bool there, int D, int g, half8 (*hi)[2], half8 (*lo)[2]) {
+    float x[NI][16];
+    float amax = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int d = 16 * (4 * i + g) + e;
+            x[i][e] = there && d < D ? key_value(row, d, std::integral_constant<int, KIND>{}) : 0.0f;
+            amax = fmaxf(amax, fabsf(x[i][e]));
+            odd = odd || !(fabsf(x[i][e]) < INFINITY);
+        }
+    amax = max_g(odd ? INFINITY : amax);
+    odd = amax == INFINITY;  // (an infinity or NaN: the key's scores are NaN, and no other key's)
+    const int e2 = exponent_of(amax);
+    const float inv = pow2(-e2);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[i][e] = odd ? 0.0f : x[i][e];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) split8(x[i] + 8 * j, inv, hi[i][j], lo[i][j]);
+    }
+    return odd ? NAN : pow2(e2);
+}
+
+// grid: (wavefronts' keys / 4, B * Hkv, column splits)
+template <typename QT, int SRC, int NI, int TW>
+__global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
+    constexpr bool CODES = SRC == kInt8 || SRC == kE4m3;
+    constexpr bool KLO = CODES || SRC == kF32 || SRC == kQ8;  // keys may need lo operands (a tail's do)
+    constexpr bool QLO = __is_same(QT, float);
+    constexpr int Dp = 64 * NI;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t bg = blockIdx.y, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
+    const int len = a.len[b], full = CODES ? len / a.N * a.N : 0;
+    const int k0 = ((int)blockIdx.x * kWaves + w) * 16 * TW;
+    if (k0 >= len) return;
+
+    half8 kh[TW][NI][2], kl[TW][NI][2];
+    float ksc[TW][4];
+    bool lo_used = !CODES && KLO;
+#pragma unroll
+    for (int kb = 0; kb < TW; ++kb) {
+        const int t0 = k0 + 16 * kb, t = t0 + n;
+        if (CODES && t0 < full) {  // (a whole block is a multiple of 16 tokens)
+            const uint8_t *p = (const uint8_t *)a.k + bg * a.units * kUnit * Dp + (int64_t)t0 * Dp + 16 * lane;
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const u32x4 r = *(const u32x4 *)(p + 1024 * i);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    kh[kb][i][j] = decode8<SRC == kE4m3>(r[2 * j], r[2 * j + 1]);
+                    kl[kb][i][j] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                }
+            }
+            const float s = a.ks[bg * (a.units * kUnit / a.N) + t0 / a.N];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ksc[kb][i] = s;
+        } else {
+            float s;
+            if constexpr (CODES) {
+                lo_used = true;
+                const int tt = t - full;
+                s = key_operands<kF32, NI>((const char *)(a.kt + (bg * a.N + tt) * a.D), t < len, a.D, g, kh[kb], kl[kb]);
+            } else {
+                s = key_operands<SRC, NI>(a.k + (bg * a.cap + t) * a.row_bytes, t < len, a.D, g, kh[kb], kl[kb]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ksc[kb][i] = __shfl(s, 4 * g + i, 64);
+        }
+    }
+
+    float sum[TW][4];
+#pragma unroll
+    for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[kb][i] = 0.0f;
+    const int G = a.H / a.Hkv, rows = G * a.L;
+    const int c0 = blockIdx.z * a.span, c1 = min(c0 + a.span, a.col_tiles);
+    for (int ct = c0; ct < c1; ++ct) {
+        const int rr = 16 * ct + n, r = min(rr, rows - 1), hh = r / a.L, l = r - hh * a.L;
+        const int lim = rr < rows ? (a.causal ? len - a.L + l + 1 : len) : 0;
+        if (__builtin_amdgcn_ballot_w64(lim > k0) == 0) continue;
+        half8 qh[NI][2], ql[NI][2];
+        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
+        const float f = load_query<QT, NI>(row, a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e;
+        const float ls = a.lse[(b * a.H + kvh * G) * a.L + r] * kLog2e;
+#pragma unroll
+        for (int kb = 0; kb < TW; ++kb) {
+            f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (QLO) c = mma(kh[kb][i][j], ql[i][j], c);
+                    if constexpr (KLO) {
+                        if (lo_used) c = mma(kl[kb][i][j], qh[i][j], c);
+                    }
+                    c = mma(kh[kb][i][j], qh[i][j], c);
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(c[i] * (f * ksc[kb][i]) - ls);
+                sum[kb][i] += k0 + 16 * kb + 4 * g + i < lim ? p : 0.0f;
+            }
+        }
+    }
+#pragma unroll
+    for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float s = sum[kb][i];
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
+            const int t = k0 + 16 * kb + 4 * g + i;
+            if (n != 0 || t >= len) continue;
+            if (a.parts) a.parts[((int64_t)blockIdx.z * gridDim.y + bg) * a.cap + t] = s;
+            else {
+                float *o = a.sums + bg * a.cap + t;
+                *o = a.keep == 0.0f ? s : fmaf(a.keep, *o, s);
+            }
+        }
+}
+
+__global__ void add_parts_kernel(const float *parts, int splits, int64_t stride, const int32_t *len, float *sums, float keep,
+                                 int Hkv, int64_t cap) {
+    const int64_t bg = blockIdx.y, t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (t >= len[bg / Hkv]) return;
+    float s = 0.0f;
+    for (int z = 0; z < splits; ++z) s += parts[z * stride + bg * cap + t];
+    float *o = sums + bg * cap + t;
+    *o = keep == 0.0f ? s : fmaf(keep, *o, s);
+}
+
+template <typename QT, int SRC>
+const void *kernel_d(int Dp) {
+    switch (Dp) {
+        case 64: return (const void *)attn_key_weights_kernel<QT, SRC, 1, 4>;
+        case 128: return (const void *)attn_key_weights_kernel<QT, SRC, 2, 4>;
+        default: return (const void *)attn_key_weights_kernel<QT, SRC, 4, 2>;
+    }
+}
+
+template <typename QT>
+const void *kernel_src(int src, int Dp) {
+    switch (src) {
+        case kInt8: return kernel_d<QT, kInt8>(Dp);
+        case kE4m3: return kernel_d<QT, kE4m3>(Dp);
+        case kF16: return kernel_d<QT, kF16>(Dp);
+        case kBf16: return kernel_d<QT, kBf16>(Dp);
+        case kF32: return kernel_d<QT, kF32>(Dp);
+        default: return kernel_d<QT, kQ8>(Dp);
+    }
+}
+
+}  // namespace
+
+hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s) {
+    if (r.B * r.Hkv > 65535 || r.D > kMaxDim) return hipErrorInvalidConfiguration;
+    Args a{};
+    a.q = r.q;
+    a.q_sb = r.q_strides[0];
+    a.q_sh = r.q_strides[1];
+    a.q_sl = r.q_strides[2];
+    a.cap = r.cap;
+    a.lse = r.lse;
+    a.len = r.len;
+    a.sums = r.sums;
+    a.keep = r.keep;
+    a.scale = r.scale;
+    a.causal = r.causal;
+    const int64_t per16 = r.q_dtype == GT_F32 ? 4 : 8;
+    a.q_vec = (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
+    a.H = (int)r.H;
+    a.Hkv = (int)r.Hkv;
+    a.L = (int)r.L;
+    a.D = (int)r.D;
+    int src;
+    if (r.blocks) {
+        src = r.blocks->e4m3 ? kE4m3 : kInt8;
+        a.k = (const char *)r.blocks->codes[0];
+        a.ks = r.blocks->scales[0];
+        a.kt = r.blocks->tail[0];
+        a.N = r.blocks->N;
+        a.units = r.blocks->units;
+    } else {
+        src = r.k_dtype == GT_F16 ? kF16 : r.k_dtype == GT_BF16 ? kBf16 : r.k_dtype == GT_F32 ? kF32 : kQ8;
+        a.k = (const char *)r.k;
+        a.row_bytes = r.k_dtype == GT_Q8_0 ? r.D / 32 * 34 : r.k_dtype == GT_F32 ? r.D * 4 : r.D * 2;
+    }
+    const int Dp = padded_dim(r.D), keys = 16 * (Dp == 256 ? 2 : 4) * kWaves;
+    const void *kernel = r.q_dtype == GT_F16   ? kernel_src<_Float16>(src, Dp)
+                         : r.q_dtype == GT_BF16 ? kernel_src<__bf16>(src, Dp)
+                                                : kernel_src<float>(src, Dp);
+    const int64_t rows = r.H / r.Hkv * r.L, tiles = (rows + 15) / 16, wgs = (r.max_len + keys - 1) / keys;
+    // column splits: towards 512 workgroups (two a CU), of 8 columns of 16 rows at least (a wavefront's keys cost
+    // about as much as four)
+    int64_t splits = std::min<int64_t>(tiles / 8, 512 / std::max<int64_t>(1, wgs * r.B * r.Hkv));
+    splits = std::max<int64_t>(1, splits);
+    a.col_tiles = (int)tiles;
+    a.span = (int)((tiles + splits - 1) / splits);
+    splits = (tiles + a.span - 1) / a.span;
+    gt_scratch parts;
+    if (splits > 1) {
+        if (!gt_scratch_alloc(parts, (size_t)(splits * r.B * r.Hkv * r.cap) * sizeof(float), dev)) return hipErrorOutOfMemory;
+        a.parts = (float *)parts.ptr();
+    }
+    void *args[] = {(void *)&a};
+    hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)wgs, (unsigned)(r.B * r.Hkv), (unsigned)splits), dim3(64 * kWaves), args, 0, s);
+    if (e != hipSuccess || splits == 1) return e;
+    hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)((r.max_len + 255) / 256), (unsigned)(r.B * r.Hkv)), dim3(256), 0, s,
+                       (const float *)a.parts, (int)splits, r.B * r.Hkv * r.cap, r.len, r.sums, r.keep, (int)r.Hkv, r.cap);
+    return hipGetLastError();
+}

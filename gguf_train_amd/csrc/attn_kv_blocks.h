@@ -1,0 +1,547 @@
+// Attention of few query rows over the 8-bit block cache (kv_blocks.h), straight from the codes: decode steps,
+// and the several tokens of a draft that are checked together.
+//
+//   s[r, t] = scale q_r . k_t,  p = softmax over the keys that row r sees,  o_r = sum_t p[r, t] v_t
+// with k_t = code x 2^a, v_t = code x 2^c, a and c a block's exponents.  HBM-bound: K and V are read once, a
+// byte a value.
+//
+// Rows: the G query heads of a kv head times the L tokens, r = head * L + token, are the columns of the matrix
+// instruction, 16 CT of them per workgroup; more take further workgroups over the same keys.  A workgroup owns
+// a span of 64-token units (a split of the sequence), its four wavefronts take them in turn, each with its own
+// running maximum and sum; they are joined once at the end, and the last split of a row group to finish joins
+// the splits (partials in uncached memory, as in decode_merge.h).
+//
+// Products on v_mfma_f32_16x16x32_f16, float32 sums.  Codes become float16 exactly: int8 by placing two bytes
+// under exponent bytes (1024 + 128 + code) and subtracting 1152, e4m3 by the hardware's conversion.
+// Score S^T = K.Q^T: float16 queries are their own operand; bfloat16 and float32 rows are scaled by a power of
+// two to a largest magnitude in [1, 2) and enter as one operand (bfloat16: exact, but for elements below 2^-14
+// of the largest, which keep 2^-25 of it) or as two, x = hi + lo (float32: off by 2^-25 of the largest).
+// P.V: the weights enter as p' = p 2^(c - r), the reference r following the largest p 2^c so that p' <= 1 and
+// what float16 loses below 2^-14 is small against the largest term, whatever the blocks' scales.  float16 and
+// bfloat16 results take p' rounded to float16 (2^-12 of each term), float32 results take hi + lo.
+//
+// The tail's float32 tokens are one or two more units: a key's row (K and V) is scaled by its own power of two
+// and split into hi + lo operands, which carry 22 bits.  A key with an infinity or NaN has codes of zero and a
+// NaN for a scale, which only the rows that see it meet.
+#pragma once
+
+#include "attn_common.h"
+#include "gt_internal.h"
+#include "kv_blocks.h"
+#include "mfma_util.h"
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <map>
+#include <mutex>
+
+namespace gtkvb {
+
+using gtmfma::fast_exp2;
+using gtmfma::half8;
+using gtmfma::f32x4;
+using gtmfma::kLn2;
+using gtmfma::kLog2e;
+using gtmfma::u32x4;
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+
+constexpr int kWaves = 4;
+
+struct AttnArgs {
+    const void *q;
+    int64_t q_sb, q_sh, q_sl;  // element strides; dims contiguous
+    void *o;                   // dense (B, H, L, D) of q's type
+    float *lse;                // (B, H, L) or null
+    const uint8_t *k, *v;
+    const float *ks, *vs, *kt, *vt;  // scales and tails
+    const int32_t *len;
+    float scale;
+    int causal, q_vec;  // q_vec: query rows in aligned 16-byte pieces
+    int B, H, Hkv, L, D, N;
+    int64_t units;  // of a slice
+    int groups;     // row groups per kv head
+    int nsplit, span;  // splits, units of each
+    float *part_o, *part_ml;  // (rows, nsplit, Dp), (rows, nsplit, 2)
+    int *counters;
+};
+
+// max over the four lanes 16 g + m of one m
+__device__ inline float max_g(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    return gtmfma::xhalf_max(v);
+}
+__device__ inline float sum_g(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    return gtmfma::xhalf_sum(v);
+}
+__device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+// e with 2^e <= a < 2^(e+1), kept within what pow2 and its reciprocal reach; 0 for a zero, infinity or NaN
+__device__ inline int exponent_of(float a) {
+    if (!(a > 0.0f) || !(a < INFINITY)) return 0;
+    return min(max((int)(__float_as_uint(a) >> 23) - 127, -126), 126);
+}
+
+// Eight codes as float16.
+template <bool E4M3>
+__device__ inline half8 decode8(uint32_t w0, uint32_t w1) {
+    half2v h[4];
+    if constexpr (E4M3) {
+        h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+        h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+        h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+        h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+    } else {
+        // bytes u = code + 128 under 0x64: 1024 + u
+        const half2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
+        w0 ^= 0x80808080u;
+        w1 ^= 0x80808080u;
+        constexpr uint32_t k64 = 0x64646464u;
+        h[0] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w0, 0x04010400u)) - off;
+        h[1] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w0, 0x04030402u)) - off;
+        h[2] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w1, 0x04010400u)) - off;
+        h[3] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w1, 0x04030402u)) - off;
+    }
+    const u32x4 r = {__builtin_bit_cast(uint32_t, h[0]), __builtin_bit_cast(uint32_t, h[1]),
+                     __builtin_bit_cast(uint32_t, h[2]), __builtin_bit_cast(uint32_t, h[3])};
+    return __builtin_bit_cast(half8, r);
+}
+
+__device__ inline f32x4 mma(half8 a, half8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// x * inv as hi (+ lo) float16
+__device__ inline void split8(const float *x, float inv, half8 &hi, half8 &lo) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float y = x[e] * inv;
+        hi[e] = (_Float16)y;
+        lo[e] = (_Float16)(y - (float)hi[e]);
+    }
+}
+
+// The B operands of one query row: lane (n, g) holds dims 16 (4i + g) .. +15 of its column's row, operand j the
+// eight from 8j on.  Returns the row's scale (the operands are the row divided by it).
+template <typename QT, int NI>
+__device__ inline float load_query(const QT *row, int D, bool vec, int g, half8 (*hi)[2], half8 (*lo)[2]) {
+    constexpr bool F16 = __is_same(QT, _Float16);
+    float x[NI][16];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int d0 = 16 * (4 * i + g);
+        if (vec && d0 + 16 <= D) {
+            struct alignas(16) P {
+                QT e[16 / sizeof(QT)];
+            };
+            constexpr int PER = 16 / sizeof(QT);
+#pragma unroll
+            for (int p = 0; p < 16 / PER; ++p) {
+                const P piece = *(const P *)(row + d0 + p * PER);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) x[i][p * PER + e] = (float)piece.e[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[i][e] = d0 + e < D ? (float)row[d0 + e] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
+    }
+    int e2 = 0;
+    if constexpr (!F16) e2 = exponent_of(max_g(amax));
+    const float inv = F16 ? 1.0f : pow2(-e2);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) split8(x[i] + 8 * j, inv, hi[i][j], lo[i][j]);
+    return pow2(e2);
+}
+
+// Joins the splits of rows row0 .. row0 + n - 1, one wavefront a row; uncached partials (see decode_merge.h).
+template <typename TO, int NI>
+__device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n) {
+    constexpr int Dp = 64 * NI;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ns = a.nsplit;
+    for (int r = w; r < n; r += kWaves) {
+        const int64_t row = row0 + r;
+        const float *ml = a.part_ml + row * ns * 2, *po = a.part_o + row * ns * Dp + lane;
+        // (max, sum) of split `lane`; at most 64 splits
+        const float mi = lane < ns ? ml[2 * lane] : -INFINITY, li = lane < ns ? ml[2 * lane + 1] : 0.0f;
+        float M = mi, L;
+        for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        const float wi = mi == -INFINITY && !(li != li) ? 0.0f : fast_exp2(mi - (M == -INFINITY ? 0.0f : M));
+        L = wi * li;
+        if (li != li) L = li;
+        for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
+        float acc[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i] = 0.0f;
+        constexpr int U = 8;
+        for (int s0 = 0; s0 < ns; s0 += U) {
+            float x[U][NI];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < NI; ++i) x[u][i] = po[(int64_t)min(s0 + u, ns - 1) * Dp + 64 * i];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float ws = s0 + u < ns ? __shfl(wi, min(s0 + u, ns - 1), 64) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < NI; ++i) acc[i] = ws == 0.0f ? acc[i] : fmaf(ws, x[u][i], acc[i]);
+            }
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            if (lane + 64 * i < a.D) ((TO *)a.o)[row * a.D + lane + 64 * i] = (TO)(acc[i] * inv);
+        if (a.lse && lane == 0) a.lse[row] = L == 0.0f ? INFINITY : (M + log2f(L)) * kLn2;
+    }
+}
+
+template <typename QT, int NI, int CT, bool E4M3>
+__global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
+    constexpr bool F32 = __is_same(QT, float);
+    constexpr int Dp = 64 * NI, COLS = 16 * CT, DT = 4 * NI;
+    constexpr int OP = Dp + 4;  // pitch of the joined rows
+    __shared__ float s_o[COLS * OP];
+    __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
+    __shared__ int s_last;
+
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t x = blockIdx.x, bg = x / a.groups, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
+    const int rg = (int)(x - bg * a.groups), G = a.H / a.Hkv, rows = G * a.L;
+    const int r0 = rg * COLS, nr = min(COLS, rows - r0);
+    const int len = a.len[b], full = len / a.N * a.N, tail = len - full;
+
+    // queries, and the first key that each column does not see
+    half8 qh[CT][NI][2], ql[CT][NI][2];
+    float f[CT];
+    int lim[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int r = r0 + min(16 * ct + n, nr - 1), hh = r / a.L, l = r - hh * a.L;
+        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
+        f[ct] = load_query<QT, NI>(row, a.D, a.q_vec, g, qh[ct], ql[ct]) * a.scale * kLog2e;
+        lim[ct] = 16 * ct + n < nr ? (a.causal ? len - a.L + l + 1 : len) : 0;
+    }
+    const int lim_all = a.causal ? len - a.L + 1 : len;  // keys below it are seen by every row
+
+    float m[CT], mv[CT], lsum[CT];  // running max of s and of s + c, sum of 2^(s - m)
+    f32x4 acc[CT][DT];              // sum of 2^(s + c - mv) code
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        m[ct] = mv[ct] = -INFINITY;
+        lsum[ct] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // The softmax step over 64 keys from k0 on: c holds the column's products with the codes of keys 16 kb + 4g + i,
+    // ksc and vexp(kb, i) a key's scale and V exponent; every key at or above `end` is not there.  Leaves p' as
+    // operands and rescales the sums.
+    auto softmax = [&](f32x4(&c)[CT][4], int k0, int end, auto &&ksc, auto &&vexp, half8(&ph)[CT][2], half8(&pl)[CT][2]) {
+        const bool all = k0 + kUnit <= min(lim_all, end) && nr == COLS;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            float cm = -INFINITY, cv = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float s = c[ct][kb][i] * (f[ct] * ksc(kb, i));
+                    if (!all) s = k0 + 16 * kb + 4 * g + i < min(lim[ct], end) ? s : -INFINITY;
+                    c[ct][kb][i] = s;
+                    cm = fmaxf(cm, s);
+                    cv = fmaxf(cv, s + vexp(kb, i));
+                }
+            const float mn = fmaxf(m[ct], max_g(cm)), vn = fmaxf(mv[ct], max_g(cv));
+            const float ms = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m[ct] - mn);
+            const float beta = vn == -INFINITY ? 1.0f : fast_exp2(mv[ct] - vn);
+            const float shift = (vn == -INFINITY ? 0.0f : vn) - ms;
+            m[ct] = mn;
+            mv[ct] = vn;
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = fast_exp2(c[ct][kb][i] - ms);
+                    sum += p;
+                    // p <= 2^-100 next to a larger 2^c: nothing of the sum; a NaN exponent (a block that holds one) stays
+                    const float e = vexp(kb, i) - shift;
+                    const float pv = p == 0.0f ? 0.0f : p * fast_exp2(e > 100.0f ? 100.0f : e);
+                    const int at = 4 * (kb & 1) + i;
+                    const _Float16 hi = (_Float16)pv;
+                    ph[ct][kb >> 1][at] = hi;
+                    if constexpr (F32) pl[ct][kb >> 1][at] = (_Float16)(pv - (float)hi);
+                }
+            lsum[ct] = fmaf(lsum[ct], alpha, sum_g(sum));
+            if (__builtin_amdgcn_ballot_w64(beta != 1.0f) != 0) {
+#pragma unroll
+                for (int t = 0; t < DT; ++t) acc[ct][t] *= beta;
+            }
+        }
+    };
+
+    // ---- whole blocks ----
+    const int u0 = blockIdx.y * a.span, u1 = min(u0 + a.span, (full + kUnit - 1) / kUnit);
+    const int64_t slice = bg * a.units * kUnit * Dp;
+    const uint8_t *kc = a.k + slice + 16 * lane, *vc = a.v + slice + 16 * lane;
+    const int64_t nblk = a.units * kUnit / a.N;
+    const float *sc = ((lane & 4) ? a.vs : a.ks) + bg * nblk;  // lanes 0..3 hold K's scales, 4..7 V's
+    u32x4 rk[DT], rv[DT];
+    float rs = 0.0f;
+    auto load_k = [&](int u) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            rk[t] = __builtin_nontemporal_load((const u32x4 *)(kc + (int64_t)u * kUnit * Dp + 1024 * t));
+        rs = sc[min((int64_t)(u * kUnit + 16 * (lane & 3)) / a.N, nblk - 1)];
+    };
+    auto load_v = [&](int u) {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+            rv[t] = __builtin_nontemporal_load((const u32x4 *)(vc + (int64_t)u * kUnit * Dp + 1024 * t));
+    };
+    f32x4 c[CT][4];
+    float sk[4], ev[4];
+    auto scores = [&]() {
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            sk[kb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rs), kb));
+            const uint32_t vb = __builtin_amdgcn_readlane(__float_as_uint(rs), 4 + kb);
+            ev[kb] = (vb >> 23) == 255 ? NAN : (float)((int)(vb >> 23) - 127);
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const half8 ka = decode8<E4M3>(rk[kb * NI + i][2 * j], rk[kb * NI + i][2 * j + 1]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        if constexpr (F32) c[ct][kb] = mma(ka, ql[ct][i][j], c[ct][kb]);
+                        c[ct][kb] = mma(ka, qh[ct][i][j], c[ct][kb]);
+                    }
+                }
+        }
+    };
+    half8 ph[CT][2], pl[CT][2];
+    auto weigh = [&](int u) {
+        softmax(c, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; }, ph, pl);
+    };
+    auto values = [&]() {
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const half8 va = decode8<E4M3>(rv[t][2 * j], rv[t][2 * j + 1]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    if constexpr (F32) acc[ct][t] = mma(va, pl[ct][j], acc[ct][t]);
+                    acc[ct][t] = mma(va, ph[ct][j], acc[ct][t]);
+                }
+            }
+    };
+    // the next unit's K is on its way during the softmax and P.V, its V during the next scores
+    int u = u0 + w;
+    if (u < u1) {
+        load_k(u);
+        load_v(u);
+        for (; u + kWaves < u1; u += kWaves) {
+            scores();
+            load_k(u + kWaves);
+            weigh(u);
+            values();
+            load_v(u + kWaves);
+        }
+        scores();
+        weigh(u);
+        values();
+    }
+
+    // ---- the tail: by the last split that has units, as its next ones ----
+    const int nu = max(u1 - u0, 0);
+    const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && u1 * kUnit >= full;
+    for (int tu = 0; mine && tu * kUnit < tail; ++tu) {
+        if ((nu + tu) % kWaves != w) continue;
+        const float *kt = a.kt + bg * a.N * a.D, *vt = a.vt + bg * a.N * a.D;
+        const int t0 = tu * kUnit;
+        float ksc[4][4], vex[4][4], vinv[4][4];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            // K row 16 kb + n of the unit; its scale goes to the lanes that hold its scores
+            const int t = t0 + 16 * kb + n;
+            float x[NI][16];
+            float amax = 0.0f;
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int d = 16 * (4 * i + g) + e;
+                    x[i][e] = t < tail && d < a.D ? kt[(int64_t)t * a.D + d] : 0.0f;
+                    amax = fmaxf(amax, fabsf(x[i][e]));
+                    odd = odd || !(fabsf(x[i][e]) < INFINITY);
+                }
+            amax = max_g(odd ? INFINITY : amax);
+            odd = amax == INFINITY;
+            const int e2 = exponent_of(amax);
+            const float inv = pow2(-e2);
+            if (odd) {
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[i][e] = 0.0f;
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    half8 hi, lo;
+                    split8(x[i] + 8 * j, inv, hi, lo);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        if constexpr (F32) c[ct][kb] = mma(hi, ql[ct][i][j], c[ct][kb]);
+                        c[ct][kb] = mma(lo, qh[ct][i][j], c[ct][kb]);
+                        c[ct][kb] = mma(hi, qh[ct][i][j], c[ct][kb]);
+                    }
+                }
+            const float ks = odd ? NAN : pow2(e2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ksc[kb][i] = __shfl(ks, 4 * g + i, 64);
+            // V rows 16 kb + 4g + i: the largest magnitude over the dims, of which this lane sees each 16th
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int tv = t0 + 16 * kb + 4 * g + i;
+                float vm = 0.0f;
+                bool vodd = false;
+                for (int d = n; d < a.D; d += 16) {
+                    const float y = tv < tail ? fabsf(vt[(int64_t)tv * a.D + d]) : 0.0f;
+                    vm = fmaxf(vm, y);
+                    vodd = vodd || !(y < INFINITY);
+                }
+                vm = vodd ? INFINITY : vm;
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) vm = fmaxf(vm, __shfl_xor(vm, o, 64));
+                const int ve = vm == 0.0f ? -126 : exponent_of(vm);
+                vex[kb][i] = vm == INFINITY ? NAN : (float)ve;
+                vinv[kb][i] = vm == INFINITY || vm == 0.0f ? 0.0f : pow2(-ve);
+            }
+        }
+        softmax(c, full + t0, len, [&](int kb, int i) { return ksc[kb][i]; }, [&](int kb, int i) { return vex[kb][i]; }, ph, pl);
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+            const int d = 16 * t + n;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                half8 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int kb = 2 * j + (e >> 2), i = e & 3, tv = t0 + 16 * kb + 4 * g + i;
+                    const bool there = tv < tail && d < a.D && vinv[kb][i] != 0.0f;
+                    const float y = there ? vt[(int64_t)tv * a.D + d] * vinv[kb][i] : 0.0f;
+                    hi[e] = (_Float16)y;
+                    lo[e] = (_Float16)(y - (float)hi[e]);
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    if constexpr (F32) acc[ct][t] = mma(hi, pl[ct][j], acc[ct][t]);
+                    acc[ct][t] = mma(lo, ph[ct][j], acc[ct][t]);
+                    acc[ct][t] = mma(hi, ph[ct][j], acc[ct][t]);
+                }
+            }
+        }
+    }
+
+    // ---- join the wavefronts, in order ----
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+        if (g == 0) {
+            s_m[w][16 * ct + n] = m[ct];
+            s_l[w][16 * ct + n] = lsum[ct];
+        }
+    __syncthreads();
+    for (int ww = 0; ww < kWaves; ++ww) {
+        if (w == ww) {
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                const int col = 16 * ct + n;
+                const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+                const float to = mv[ct] == -INFINITY ? 0.0f : fast_exp2(mv[ct] - (M == -INFINITY ? 0.0f : M));
+                const bool bad = lsum[ct] != lsum[ct];
+#pragma unroll
+                for (int t = 0; t < DT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float *o = &s_o[col * OP + 16 * t + 4 * g + i];
+                        const float y = bad ? NAN : acc[ct][t][i] * to;
+                        *o = ww == 0 ? y : *o + y;
+                    }
+            }
+        }
+        __syncthreads();
+    }
+    const int64_t row0 = (b * a.H + kvh * G) * a.L + r0;
+    for (int e = threadIdx.x; e < nr * Dp; e += 64 * kWaves) {
+        const int col = e / Dp, d = e - col * Dp;
+        const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+        float L = 0.0f;
+#pragma unroll
+        for (int ww = 0; ww < kWaves; ++ww) {
+            const float lw = s_l[ww][col];
+            L += s_m[ww][col] == -INFINITY ? (lw != lw ? lw : 0.0f) : fast_exp2(s_m[ww][col] - M) * lw;
+        }
+        const float o = s_o[col * OP + d];
+        const int64_t row = row0 + col;
+        if (a.nsplit == 1) {
+            if (d < a.D) ((QT *)a.o)[row * a.D + d] = (QT)(L == 0.0f ? 0.0f : o / L);
+            if (a.lse && d == 0) a.lse[row] = L == 0.0f ? INFINITY : (M + log2f(L)) * kLn2;
+        } else {
+            const int64_t pr = row * a.nsplit + blockIdx.y;
+            a.part_o[pr * Dp + d] = o;
+            if (d == 0) {
+                a.part_ml[2 * pr] = M;
+                a.part_ml[2 * pr + 1] = L;
+            }
+        }
+    }
+    if (a.nsplit == 1) return;
+    // every split writes its partial; the last one to arrive joins them (partials and counters are uncached)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(&a.counters[x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.nsplit - 1;
+    __syncthreads();
+    if (!s_last) return;
+    merge_splits<QT, NI>(a, row0, nr);
+    if (threadIdx.x == 0) __hip_atomic_store(&a.counters[x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The kernel for head sizes padded to Dp and up to 16 ct rows a workgroup; null when there is none (ct Dp / 64
+// <= 4: past it the sums of P.V and the queries do not stay in registers).
+template <typename QT>
+inline const void *attn_kernel(int Dp, int ct, bool e4m3) {
+#define GT_K(NI, CT) (e4m3 ? (const void *)attn_kv_blocks_kernel<QT, NI, CT, true> : (const void *)attn_kv_blocks_kernel<QT, NI, CT, false>)
+    switch (Dp / 64 * 10 + ct) {
+        case 11: return GT_K(1, 1);
+        case 12: return GT_K(1, 2);
+        case 14: return GT_K(1, 4);
+        case 21: return GT_K(2, 1);
+        case 22: return GT_K(2, 2);
+        case 41: return GT_K(4, 1);
+        default: return nullptr;
+    }
+#undef GT_K
+}
+
+const void *attn_kernel_f16(int Dp, int ct, bool e4m3);
+const void *attn_kernel_bf16(int Dp, int ct, bool e4m3);
+const void *attn_kernel_f32(int Dp, int ct, bool e4m3);
+
+}  // namespace gtkvb

@@ -1,0 +1,103 @@
+// Launches of the attention over the 8-bit block cache (attn_kv_blocks.h).
+
+#include "attn_kv_blocks.h"
+
+#include <cmath>
+#include <string>
+
+namespace {
+
+using namespace gtkvb;
+
+const void *kernel_of(int q_dtype, int Dp, int ct, bool e4m3) {
+    switch (q_dtype) {
+        case GT_F16: return attn_kernel_f16(Dp, ct, e4m3);
+        case GT_BF16: return attn_kernel_bf16(Dp, ct, e4m3);
+        case GT_F32: return attn_kernel_f32(Dp, ct, e4m3);
+        default: return nullptr;
+    }
+}
+
+// Workgroups of `kernel` the device runs at once.
+int64_t resident_groups(const void *kernel) {
+    static std::mutex mu;
+    static std::map<std::pair<int, const void *>, int64_t> known;
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = known.find({dev, kernel});
+    if (it != known.end()) return it->second;
+    int cus = 0, per = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * kWaves, 0) != hipSuccess || per <= 0) per = 1;
+    return known[{dev, kernel}] = (int64_t)cus * per;
+}
+
+}  // namespace
+
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype) {
+    const int64_t rows = H / c.Hkv * L;
+    return (q_dtype == GT_F16 || q_dtype == GT_BF16 || q_dtype == GT_F32) && rows <= kKvBlocksAttnRows &&
+           c.B * H * L < (1LL << 31);
+}
+
+hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note) {
+    AttnArgs a{};
+    a.q = r.q;
+    a.q_sb = r.q_strides[0];
+    a.q_sh = r.q_strides[1];
+    a.q_sl = r.q_strides[2];
+    a.o = r.o;
+    a.lse = r.lse;
+    a.k = (const uint8_t *)c.codes[0];
+    a.v = (const uint8_t *)c.codes[1];
+    a.ks = c.scales[0];
+    a.vs = c.scales[1];
+    a.kt = c.tail[0];
+    a.vt = c.tail[1];
+    a.len = r.len;
+    a.scale = r.scale;
+    a.causal = r.causal;
+    const int64_t per16 = r.q_dtype == GT_F32 ? 4 : 8;
+    a.q_vec = (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
+    a.B = (int)c.B;
+    a.H = (int)r.H;
+    a.Hkv = (int)c.Hkv;
+    a.L = (int)r.L;
+    a.D = (int)c.D;
+    a.N = c.N;
+    a.units = c.units;
+    // columns of a workgroup: the fewest that hold the rows, as many as the head size allows
+    const int64_t rows = r.H / c.Hkv * r.L;
+    int ct = 1;
+    while (16 * ct < rows && 2 * ct * (c.Dp / 64) <= 4) ct *= 2;
+    a.groups = (int)((rows + 16 * ct - 1) / (16 * ct));
+    const void *kernel = kernel_of(r.q_dtype, c.Dp, ct, c.e4m3);
+    if (!kernel) return hipErrorInvalidValue;
+    const int64_t grid = c.B * c.Hkv * a.groups;
+    if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
+    // splits: a workgroup's four wavefronts take a unit each per step
+    const int64_t units = (r.max_len / c.N * c.N + kUnit - 1) / kUnit, steps = std::max<int64_t>(1, (units + kWaves - 1) / kWaves);
+    int n = decode_split_count(grid, steps, resident_groups(kernel), std::min<int64_t>(64, steps));
+    int64_t per = (steps + n - 1) / n;
+    n = (int)((steps + per - 1) / per);
+    gt_decode_ws ws{};
+    if (n > 1) {
+        const size_t out_rows = (size_t)(c.B * r.H * r.L) * (size_t)n;
+        if (gt_decode_workspace(dev, s, grid, out_rows * (size_t)(c.Dp + 2) * sizeof(float), ws)) {
+            a.counters = ws.counters;
+            a.part_o = (float *)ws.parts;
+            a.part_ml = a.part_o + out_rows * (size_t)c.Dp;
+        } else {
+            n = 1;  // (no workspace for this stream, or a batch that fills the GPU without splits)
+            per = steps;
+        }
+    }
+    a.nsplit = n;
+    a.span = (int)(per * kWaves);
+    note = std::string("decode ") + (c.e4m3 ? "e4m3" : "int8") + " blocks of " + std::to_string(c.N) + " D=" + std::to_string(c.D) +
+           " rows=" + std::to_string(rows) + " columns=" + std::to_string(16 * ct) + " splits=" + std::to_string(n) +
+           " units=" + std::to_string(grid);
+    void *args[] = {(void *)&a};
+    return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3(64 * kWaves), args, 0, s);
+}

@@ -7,10 +7,13 @@
 
 #include "attn_common.h"
 #include "gt_internal.h"
+#include "kv_blocks.h"
 
 #include <algorithm>
 #include <cmath>
 #include <cstdlib>
+#include <exception>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1339,7 +1342,9 @@ extern "C" gt_tensor *gt_attention_weights_dropout(const gt_tensor *q, const gt_
 // attends to its own position and everything before it.  Here the cache lives in HBM as dense
 // (B, Hkv, capacity, D) tensors, float16/bfloat16/float32 or GGUF Q8_0 (quantized on append
 // with the same steps as gt_quantize), with per-sequence lengths; attention over it runs the
-// same kernels as gt_flash_attention, given each sequence's length and query position.
+// same kernels as gt_flash_attention, given each sequence's length and query position.  A block cache keeps
+// 8-bit codes with a scale per block of tokens and head instead (kv_blocks.h).  Tokens can be evicted, by the
+// attention weight that they have accumulated; positions then run ahead of the lengths.
 
 struct gt_kv_cache {
     int64_t B = 0, Hkv = 0, cap = 0, D = 0;
@@ -1350,9 +1355,33 @@ struct gt_kv_cache {
     // device copy of len (int32, B), and the array that the next append writes the new lengths to (its
     // workgroups still read the old ones); the two swap, so nothing is uploaded
     gt_tensor *len_dev = nullptr, *len_next = nullptr;
+    // a block cache (dtype GT_I8 or GT_F8E4M3; k and v null): tokens per block, and per K and V the codes (B, Hkv,
+    // 64 units, Dp), the scales (B, Hkv, blocks) and the tail (B, Hkv, block, D)
+    int block = 0, Dp = 0;
+    int64_t units = 0;
+    gt_tensor *codes[2] = {}, *scales[2] = {}, *tail[2] = {};
+    int src_dtype = -1;  // the dtype of every row appended since the cache was empty (GT_F32: several)
+    // the position after each sequence's last token: len and the evicted tokens; on the device (as len) once
+    // there are any
+    std::vector<int32_t> seen;
+    gt_tensor *seen_dev = nullptr, *seen_next = nullptr;
+    gt_tensor *sums = nullptr;  // accumulated attention weights (B, Hkv, cap) float32, zeros past the lengths
 };
 
 namespace {
+
+// The body of a C entry: what it throws (std::bad_alloc) becomes an error.
+template <typename R, typename F>
+R guarded(R failed, F &&body) {
+    try {
+        return body();
+    } catch (const std::exception &e) {
+        gt_set_error(std::string("out of host memory or worse: ") + e.what());
+    } catch (...) {
+        gt_set_error("unknown C++ exception");
+    }
+    return failed;
+}
 
 bool kv_zero(gt_tensor *t) {
     return gt_hip_check(gt_launch_fill_zero(gt_data(t), (int64_t)gt_dtype_nbytes(t->dtype, t->numel), gt_stream()),
@@ -1419,6 +1448,7 @@ extern "C" gt_kv_cache *gt_kv_cache_create(int64_t batch, int64_t n_head_kv, int
     c->dtype = dtype;
     c->dev = device_index;
     c->len.assign((size_t)batch, 0);
+    c->seen.assign((size_t)batch, 0);
     const int64_t sh[4] = {batch, n_head_kv, capacity, head_dim}, lsh[1] = {batch};
     c->k = gt_new_tensor(4, sh, dtype, GT_DEV_CUDA, device_index);
     c->v = c->k ? gt_new_tensor(4, sh, dtype, GT_DEV_CUDA, device_index) : nullptr;
@@ -1432,12 +1462,67 @@ extern "C" gt_kv_cache *gt_kv_cache_create(int64_t batch, int64_t n_head_kv, int
     return c;
 }
 
+extern "C" gt_kv_cache *gt_kv_cache_create_blocks(int64_t batch, int64_t n_head_kv, int64_t capacity, int64_t head_dim,
+                                                  int dtype, int block_tokens, int device_index) {
+    return guarded((gt_kv_cache *)nullptr, [&]() -> gt_kv_cache * {
+        gt_init();
+        const std::string who = "kv_cache_create_blocks: ";
+        if (batch < 1 || n_head_kv < 1 || capacity < 1 || head_dim < 1) {
+            gt_set_error(who + "batch, n_head_kv, capacity and head_dim must be positive");
+            return nullptr;
+        }
+        if (dtype != GT_I8 && dtype != GT_F8E4M3) {
+            gt_set_error(who + "dtype must be int8 or float8_e4m3, got " + gt_dtype_name(dtype));
+            return nullptr;
+        }
+        if (block_tokens != 32 && block_tokens != 64 && block_tokens != 128) {
+            gt_set_error(who + "block_tokens must be 32, 64 or 128, got " + std::to_string(block_tokens));
+            return nullptr;
+        }
+        if (head_dim > gtkvb::kMaxDim) {
+            gt_set_error(who + "head_dim must be at most 256, got " + std::to_string(head_dim));
+            return nullptr;
+        }
+        if (capacity >= (1LL << 30) || batch > 65535 || n_head_kv > 65535 || batch * n_head_kv > 65535) {
+            gt_set_error(who + "capacity must be below 2^30, batch * n_head_kv at most 65535");
+            return nullptr;
+        }
+        if (!gt_device_ok(device_index)) return nullptr;
+        std::unique_ptr<gt_kv_cache, void (*)(gt_kv_cache *)> c(new gt_kv_cache(), gt_kv_cache_free);
+        c->B = batch;
+        c->Hkv = n_head_kv;
+        c->cap = capacity;
+        c->D = head_dim;
+        c->dtype = dtype;
+        c->dev = device_index;
+        c->block = block_tokens;
+        c->Dp = gtkvb::padded_dim(head_dim);
+        // (whole blocks of the largest size, so that every block's scale and codes have a place)
+        const int64_t tokens = (capacity + gtkvb::kMaxBlock - 1) / gtkvb::kMaxBlock * gtkvb::kMaxBlock;
+        c->units = tokens / gtkvb::kUnit;
+        c->len.assign((size_t)batch, 0);
+        c->seen.assign((size_t)batch, 0);
+        const int64_t csh[4] = {batch, n_head_kv, tokens, c->Dp}, ssh[3] = {batch, n_head_kv, tokens / block_tokens};
+        const int64_t tsh[4] = {batch, n_head_kv, block_tokens, head_dim}, lsh[1] = {batch};
+        for (int i = 0; i < 2; ++i) {
+            if (!(c->codes[i] = gt_new_tensor(4, csh, GT_U8, GT_DEV_CUDA, device_index)) ||
+                !(c->scales[i] = gt_new_tensor(3, ssh, GT_F32, GT_DEV_CUDA, device_index)) ||
+                !(c->tail[i] = gt_new_tensor(4, tsh, GT_F32, GT_DEV_CUDA, device_index)) || !kv_zero(c->codes[i]) ||
+                !kv_zero(c->scales[i]) || !kv_zero(c->tail[i]))
+                return nullptr;  // (codes of tokens not yet written meet weights of 0: no NaN among them)
+        }
+        if (!(c->len_dev = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, device_index)) ||
+            !(c->len_next = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, device_index)) || !kv_zero(c->len_dev))
+            return nullptr;
+        return c.release();
+    });
+}
+
 extern "C" void gt_kv_cache_free(gt_kv_cache *c) {
     if (!c) return;
-    gt_tensor_free(c->k);
-    gt_tensor_free(c->v);
-    gt_tensor_free(c->len_dev);
-    gt_tensor_free(c->len_next);
+    for (gt_tensor *t : {c->k, c->v, c->len_dev, c->len_next, c->codes[0], c->codes[1], c->scales[0], c->scales[1], c->tail[0],
+                         c->tail[1], c->seen_dev, c->seen_next, c->sums})
+        gt_tensor_free(t);
     delete c;
 }
 
@@ -1453,13 +1538,19 @@ extern "C" int gt_kv_cache_clear(gt_kv_cache *c, int64_t seq) {
     }
     if (!gt_device_ok(c->dev)) return -1;
     int32_t *len = (int32_t *)gt_data(c->len_dev);
-    if (seq < 0) std::fill(c->len.begin(), c->len.end(), 0);
-    else c->len[(size_t)seq] = 0;
-    return gt_hip_check(gt_launch_fill_zero(seq < 0 ? len : len + seq, (seq < 0 ? c->B : 1) * (int64_t)sizeof(int32_t),
-                                            gt_stream()),
-                        "kv cache clear kernel")
-               ? 0
-               : -1;
+    for (auto *n : {&c->len, &c->seen}) {
+        if (seq < 0) std::fill(n->begin(), n->end(), 0);
+        else (*n)[(size_t)seq] = 0;
+    }
+    if (*std::max_element(c->len.begin(), c->len.end()) == 0) c->src_dtype = -1;
+    const int64_t n = seq < 0 ? c->B : 1, from = seq < 0 ? 0 : seq;
+    auto zero = [&](void *base, int64_t bytes) {
+        return gt_hip_check(gt_launch_fill_zero((char *)base + from * bytes, n * bytes, gt_stream()), "kv cache clear kernel");
+    };
+    if (!zero(len, sizeof(int32_t))) return -1;
+    if (c->seen_dev && !zero(gt_data(c->seen_dev), sizeof(int32_t))) return -1;
+    if (c->sums && !zero(gt_data(c->sums), c->Hkv * c->cap * (int64_t)sizeof(float))) return -1;
+    return 0;
 }
 
 extern "C" int64_t gt_kv_cache_length(const gt_kv_cache *c, int64_t seq) {
@@ -1470,11 +1561,23 @@ extern "C" int64_t gt_kv_cache_length(const gt_kv_cache *c, int64_t seq) {
     return c->len[(size_t)seq];
 }
 
+extern "C" int64_t gt_kv_cache_position(const gt_kv_cache *c, int64_t seq) {
+    if (!c || seq < 0 || seq >= c->B) {
+        gt_set_error("kv_cache_position: invalid cache or sequence");
+        return -1;
+    }
+    return c->seen[(size_t)seq];
+}
+
 extern "C" int64_t gt_kv_cache_capacity(const gt_kv_cache *c) { return c ? c->cap : -1; }
 
 extern "C" gt_tensor *gt_kv_cache_keys(const gt_kv_cache *c) {
     if (!c) {
         gt_set_error("kv_cache_keys: NULL cache");
+        return nullptr;
+    }
+    if (c->block) {
+        gt_set_error("kv_cache_keys: a block cache holds codes, not rows of one dtype (see kv_cache_read)");
         return nullptr;
     }
     auto *t = new gt_tensor(*c->k);  // shares the storage
@@ -1484,6 +1587,10 @@ extern "C" gt_tensor *gt_kv_cache_keys(const gt_kv_cache *c) {
 extern "C" gt_tensor *gt_kv_cache_values(const gt_kv_cache *c) {
     if (!c) {
         gt_set_error("kv_cache_values: NULL cache");
+        return nullptr;
+    }
+    if (c->block) {
+        gt_set_error("kv_cache_values: a block cache holds codes, not rows of one dtype (see kv_cache_read)");
         return nullptr;
     }
     auto *t = new gt_tensor(*c->v);
@@ -1497,8 +1604,81 @@ struct KvRope {
     float freq_base, freq_scale;
 };
 
-// Appends k/v rows at each sequence's length; with `rope` the key rows are rotated at their cache
-// positions (length + t) on the way in.
+gt_kv_blocks kv_blocks_of(const gt_kv_cache *c) {
+    gt_kv_blocks r{};
+    for (int i = 0; i < 2; ++i) {
+        r.codes[i] = gt_data(c->codes[i]);
+        r.scales[i] = (float *)gt_data(c->scales[i]);
+        r.tail[i] = (float *)gt_data(c->tail[i]);
+    }
+    r.B = c->B;
+    r.Hkv = c->Hkv;
+    r.D = c->D;
+    r.units = c->units;
+    r.N = c->block;
+    r.Dp = c->Dp;
+    r.e4m3 = c->dtype == GT_F8E4M3;
+    return r;
+}
+
+// T tokens have been appended to every sequence, the new lengths written to len_next.
+int kv_advance(gt_kv_cache *c, int64_t T) {
+    std::swap(c->len_dev, c->len_next);
+    for (auto &n : c->len) n += (int32_t)T;
+    for (auto &n : c->seen) n += (int32_t)T;
+    if (c->seen_dev) {
+        if (!gt_hip_check(gt_launch_kv_advance((const int32_t *)gt_data(c->seen_dev), (int32_t *)gt_data(c->seen_next), T, c->B,
+                                               gt_stream()),
+                          "kv cache positions kernel"))
+            return -1;
+        std::swap(c->seen_dev, c->seen_next);
+    }
+    return 0;
+}
+
+// Appends to a block cache (arguments checked): the rows as float32, float16 or bfloat16, of one dtype.
+int kv_blocks_append(gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int64_t T, const KvRope *rope) {
+    Temps tmp;
+    const int32_t *pos = (const int32_t *)gt_data(c->len_dev);
+    const gt_tensor *src[2] = {k, v};
+    for (const gt_tensor *&t : src) {
+        if (t->dtype == GT_Q8_0) t = tmp.keep(gt_dequantize(t, GT_F32));
+        if (t && !(t->device_type == GT_DEV_CUDA && t->device_index == c->dev)) t = tmp.keep(gt_to_device_dense(t, c->dev, -1));
+        if (!t) return -1;
+    }
+    gt_scratch table;
+    if (rope) {
+        const float theta_scale = gt_rope_theta_scale(rope->freq_base, rope->n_dims);
+        const int32_t *base = c->seen_dev ? (const int32_t *)gt_data(c->seen_dev) : pos;
+        const int64_t sh[4] = {c->B, c->Hkv, T, c->D};
+        gt_tensor *turned = tmp.keep(gt_new_tensor(4, sh, src[0]->dtype, GT_DEV_CUDA, c->dev));
+        if (!turned || !gt_scratch_alloc(table, (size_t)(c->B * T) * (size_t)rope->n_dims * sizeof(float), c->dev) ||
+            !gt_hip_check(gt_launch_rope_table(nullptr, base, T, c->B * T, rope->n_dims, theta_scale, rope->freq_scale, 0, table.ptr(),
+                                               gt_stream()),
+                          "rope table kernel") ||
+            !gt_hip_check(gt_launch_rope(gt_data(src[0]), src[0]->dtype, src[0]->strides, gt_data(turned), table.ptr(), T, c->B, c->Hkv,
+                                         T, c->D, rope->n_dims, rope->mode, gt_stream()),
+                          "rope kernel"))
+            return -1;
+        src[0] = turned;
+    }
+    const bool one = src[0]->dtype == src[1]->dtype && src[0]->dtype != GT_F64;
+    for (const gt_tensor *&t : src)
+        if (!one && t->dtype != GT_F32 && !(t = tmp.keep(gt_to_device_dense(t, c->dev, GT_F32)))) return -1;
+    int64_t blocks = 0;
+    for (int32_t n : c->len) blocks = std::max<int64_t>(blocks, (n + T) / c->block - n / c->block);
+    const void *data[2] = {gt_data(src[0]), gt_data(src[1])};
+    const int64_t *strides[2] = {src[0]->strides, src[1]->strides};
+    if (!gt_hip_check(gt_launch_kv_blocks_append(kv_blocks_of(c), data, src[0]->dtype, strides, pos, nullptr,
+                                                 (int32_t *)gt_data(c->len_next), T, blocks, gt_stream()),
+                      "kv cache block append kernel"))
+        return -1;
+    c->src_dtype = c->src_dtype < 0 || c->src_dtype == src[0]->dtype ? src[0]->dtype : GT_F32;
+    return kv_advance(c, T);
+}
+
+// Appends k/v rows at each sequence's length; with `rope` the key rows are rotated at their positions (the
+// sequence's next + t) on the way in.
 int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int64_t pos_offset,
               const KvRope *rope) {
     if (!c) {
@@ -1514,15 +1694,20 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
         return -1;
     }
     for (int64_t b = 0; b < c->B; ++b) {
-        const int64_t n = c->len[(size_t)b];
-        const int64_t p0 = pos_offset < 0 ? n : pos_offset;
-        if (pos_offset >= 0 && pos_offset != n) {
+        // n tokens held, the next one's position `seen` (ahead of n once tokens have been evicted)
+        const int64_t n = c->len[(size_t)b], seen = c->seen[(size_t)b];
+        const int64_t p0 = pos_offset < 0 ? seen : pos_offset;
+        if (pos_offset >= 0 && pos_offset != seen) {
             gt_set_error("kv_cache_append: positions " + std::to_string(p0) + ".." + std::to_string(p0 + T - 1) +
-                         " do not continue what sequence " + std::to_string(b) + " holds (" + std::to_string(n) +
+                         " do not continue what sequence " + std::to_string(b) + " holds (" + std::to_string(seen) +
                          " tokens; see kv_cache_clear)");
             return -1;
         }
-        if (p0 + T > c->cap) {
+        if (seen + T > 0x7fffffffLL) {
+            gt_set_error("kv_cache_append: positions past 2^31 - 1");
+            return -1;
+        }
+        if (n + T > c->cap) {
             gt_set_error("kv_cache_append: positions " + std::to_string(p0) + ".." + std::to_string(p0 + T - 1) +
                          " of sequence " + std::to_string(b) + " do not fit the cache (capacity = " +
                          std::to_string(c->cap) + ")");
@@ -1531,9 +1716,11 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
     }
     if (!gt_device_ok(c->dev)) return -1;
     if (T == 0) return 0;
+    if (c->block) return kv_blocks_append(c, k, v, T, rope);
     Temps tmp;
     const int32_t *pos = (const int32_t *)gt_data(c->len_dev);
     int32_t *next = (int32_t *)gt_data(c->len_next);
+    const int32_t *angle_pos = c->seen_dev ? (const int32_t *)gt_data(c->seen_dev) : pos;
     gt_scratch table;
     // keys and values of one half or float32 dtype in aligned rows: one launch, which also forms the
     // angles of a few rows and the lengths after it
@@ -1544,10 +1731,10 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
                       gt_kv_append_vec_ok(gt_data(k), k->dtype, k->strides, gt_data(c->k), c->dtype, c->Hkv, T, c->D, n_dims) &&
                       gt_kv_append_vec_ok(gt_data(v), v->dtype, v->strides, gt_data(c->v), c->dtype, c->Hkv, T, c->D, 0);
     gt_rope_apply ra{};
-    if (rope && !(pair && gt_kv_rope_inline(c->B, c->Hkv, T, c->D))) {
-        // (cos, sin) of table row b * T + t at position len[b] + t
+    if (rope && !(pair && !c->seen_dev && gt_kv_rope_inline(c->B, c->Hkv, T, c->D))) {
+        // (cos, sin) of table row b * T + t at the position of sequence b's next token + t
         if (!gt_scratch_alloc(table, (size_t)(c->B * T) * (size_t)(rope->n_dims / 2) * 2 * sizeof(float), c->dev) ||
-            !gt_hip_check(gt_launch_rope_table(nullptr, pos, T, c->B * T, rope->n_dims,
+            !gt_hip_check(gt_launch_rope_table(nullptr, angle_pos, T, c->B * T, rope->n_dims,
                                                gt_rope_theta_scale(rope->freq_base, rope->n_dims), rope->freq_scale, 0,
                                                table.ptr(), gt_stream()),
                           "rope table kernel"))
@@ -1584,9 +1771,7 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
         if (!gt_hip_check(e, "kv cache append kernel")) return -1;
     }
     if (!pair && !gt_hip_check(gt_launch_kv_advance(pos, next, T, c->B, gt_stream()), "kv cache lengths kernel")) return -1;
-    std::swap(c->len_dev, c->len_next);
-    for (auto &n : c->len) n += (int32_t)T;
-    return 0;
+    return kv_advance(c, T);
 }
 
 }  // namespace
@@ -1601,8 +1786,10 @@ extern "C" int gt_kv_cache_append_rope(gt_kv_cache *c, const gt_tensor *k, const
     return kv_append("kv_cache_append_rope", c, k, v, pos_offset, &r);
 }
 
-extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal) {
-    LaunchScope scope;
+namespace {
+
+// gt_kv_cache_attention; with `lse` (float32, float16 and bfloat16 q) also the rows' log-sum-exp.
+gt_tensor *kv_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal, gt_tensor *lse) {
     if (!c) {
         gt_set_error("kv_cache_attention: NULL cache");
         return nullptr;
@@ -1640,8 +1827,33 @@ extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, 
     Temps tmp;
     bool ok = true;
     int q8 = 0;
+    if (c->block && o->numel > 0) {
+        const gt_kv_blocks blocks = kv_blocks_of(c);
+        if (gt_kv_blocks_attn_supported(blocks, H, L, q->dtype)) {
+            const gt_tensor *qs = stage(q, dev, q->dtype, tmp);
+            ok = qs != nullptr;
+            if (ok) {
+                gt_kv_blocks_attn r{};
+                r.q = gt_data(qs);
+                r.o = gt_data(o);
+                r.lse = lse ? (float *)gt_data(lse) : nullptr;
+                r.len = kv_len;
+                for (int i = 0; i < 3; ++i) r.q_strides[i] = qs->strides[i];
+                r.H = H;
+                r.L = L;
+                r.max_len = maxlen;
+                r.q_dtype = q->dtype;
+                r.causal = is_causal ? 1 : 0;
+                r.scale = scale;
+                std::string note;
+                ok = gt_hip_check(gt_launch_kv_blocks_attn(blocks, r, dev, gt_stream(), note), "kv cache block attention kernel");
+                note_launch(note);
+            }
+            q8 = 1;
+        }
+    }
     if (o->numel > 0 && c->dtype == GT_Q8_0 && q->dtype != GT_F64 && L == 1) {
-        q8 = run_q8_decode(q, c->k, c->v, nullptr, scale, is_causal, dev, o, nullptr, tmp, kv_len);
+        q8 = run_q8_decode(q, c->k, c->v, nullptr, scale, is_causal, dev, o, lse, tmp, kv_len);
         ok = q8 >= 0;
     }
     if (ok && q8 == 0 && o->numel > 0) {
@@ -1650,7 +1862,18 @@ extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, 
         // kernels run) or to float32 / float64 (exact values), as gt_flash_attention does
         const gt_tensor *kv_views[2] = {nullptr, nullptr};
         const int64_t vsh[4] = {B, c->Hkv, maxlen, D};
-        if (c->dtype == GT_Q8_0) {
+        if (c->block) {
+            // the values, which float16 and bfloat16 hold exactly; the tail's as they came, so in their dtype
+            const int kd = q->dtype == c->src_dtype ? q->dtype : GT_F32;
+            note_launch("read block cache");
+            gt_tensor *rk = tmp.keep(gt_new_tensor(4, vsh, kd, GT_DEV_CUDA, dev));
+            gt_tensor *rv = tmp.keep(gt_new_tensor(4, vsh, kd, GT_DEV_CUDA, dev));
+            ok = rk && rv &&
+                 gt_hip_check(gt_launch_kv_blocks_read(kv_blocks_of(c), kv_len, nullptr, maxlen, gt_data(rk), gt_data(rv), kd, gt_stream()),
+                              "kv cache block read kernel");
+            kv_views[0] = rk;
+            kv_views[1] = rv;
+        } else if (c->dtype == GT_Q8_0) {
             const int kd = q->dtype == GT_F16 ? GT_F16 : q->dtype == GT_F64 ? GT_F64 : GT_F32;
             note_launch("dequantize q8_0 cache rows");
             for (int i = 0; i < 2 && ok; ++i) {
@@ -1669,7 +1892,7 @@ extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, 
             }
         }
         const gt_tensor *kv = kv_views[0], *vv = kv_views[1];
-        ok = kv && vv;
+        ok = ok && kv && vv;
         const int cd = ok ? compute_dtype(q, kv, vv) : GT_F32;
         const gt_tensor *qs = ok ? stage(q, dev, cd, tmp) : nullptr;
         const gt_tensor *ks = ok ? stage(kv, dev, cd, tmp) : nullptr;
@@ -1704,6 +1927,7 @@ extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, 
             a.scale = scale;
             a.causal = is_causal ? 1 : 0;
             a.out_dtype = q->dtype;
+            a.lse = lse ? gt_data(lse) : nullptr;
             a.kv_len = kv_len;
             a.q_tail = 1;
             ok = dispatch_forward(a, cd, dev);
@@ -1715,4 +1939,269 @@ extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, 
         return nullptr;
     }
     return deliver(o, host_io);
+}
+
+// The accumulated weights, made at their first use.
+gt_tensor *kv_sums(gt_kv_cache *c) {
+    if (!c->sums) {
+        const int64_t sh[3] = {c->B, c->Hkv, c->cap};
+        gt_tensor *t = gt_new_tensor(3, sh, GT_F32, GT_DEV_CUDA, c->dev);
+        if (!t || !kv_zero(t)) {
+            gt_tensor_free(t);
+            return nullptr;
+        }
+        c->sums = t;
+    }
+    return c->sums;
+}
+
+gt_tensor *kv_attention_accumulate(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal, float keep) {
+    const std::string who = "kv_cache_attention_accumulate: ";
+    if (!(keep >= 0.0f && keep <= 1.0f)) {
+        gt_set_error(who + "the factor on the weights so far must be in [0, 1]");
+        return nullptr;
+    }
+    if (c && c->D > gtkvb::kMaxDim) {
+        gt_set_error(who + "head_dim must be at most 256, got " + std::to_string(c->D));
+        return nullptr;
+    }
+    if (c && c->B * c->Hkv > 65535) {
+        gt_set_error(who + "batch * n_head_kv must be at most 65535");
+        return nullptr;
+    }
+    if (q && (q->dtype == GT_F64 || q->ndim != 4 || q->shape[2] < 1)) {
+        gt_set_error(who + "q must be float32, float16 or bfloat16 (B, H, L, D) with at least one row");
+        return nullptr;
+    }
+    if (!c || !q) return kv_attention(c, q, scale, is_causal, nullptr);  // (its messages)
+    if (!gt_device_ok(c->dev) || !kv_sums(c)) return nullptr;
+    Temps tmp;
+    const int64_t lsh[3] = {c->B, q->shape[1], q->shape[2]};
+    gt_tensor *lse = tmp.keep(gt_new_tensor(3, lsh, GT_F32, GT_DEV_CUDA, c->dev));
+    if (!lse) return nullptr;
+    gt_tensor *o = kv_attention(c, q, scale, is_causal, lse);
+    if (!o) return nullptr;
+    const gt_tensor *qs = stage(q, c->dev, q->dtype, tmp);
+    const gt_kv_blocks blocks = c->block ? kv_blocks_of(c) : gt_kv_blocks{};
+    gt_key_weights r{};
+    if (qs) {
+        r.q = gt_data(qs);
+        r.k = c->block ? nullptr : gt_data(c->k);
+        r.blocks = c->block ? &blocks : nullptr;
+        r.lse = (const float *)gt_data(lse);
+        r.len = (const int32_t *)gt_data(c->len_dev);
+        r.sums = (float *)gt_data(c->sums);
+        for (int i = 0; i < 3; ++i) r.q_strides[i] = qs->strides[i];
+        r.B = c->B;
+        r.H = q->shape[1];
+        r.Hkv = c->Hkv;
+        r.L = q->shape[2];
+        r.D = c->D;
+        r.cap = c->cap;
+        r.max_len = *std::max_element(c->len.begin(), c->len.end());
+        r.q_dtype = q->dtype;
+        r.k_dtype = c->dtype;
+        r.causal = is_causal ? 1 : 0;
+        r.scale = scale <= 0.0f ? 1.0f / std::sqrt((float)c->D) : scale;
+        r.keep = keep;
+        note_launch("key weights");
+    }
+    if (!qs || !gt_hip_check(gt_launch_key_weights(r, c->dev, gt_stream()), "kv cache key weights kernel")) {
+        gt_tensor_free(o);
+        return nullptr;
+    }
+    return o;
+}
+
+// Evicts; `weights` null: the accumulated ones.  The kept tokens' places as *kept_out when it is given.
+int kv_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weights, gt_tensor **kept_out) {
+    const std::string who = "kv_cache_evict: ";
+    if (kept_out) *kept_out = nullptr;
+    if (!c) {
+        gt_set_error(who + "NULL cache");
+        return -1;
+    }
+    if (keep < 1 || keep > c->cap || recent < 0 || recent > keep) {
+        gt_set_error(who + "keep must be in [1, capacity = " + std::to_string(c->cap) + "] and recent in [0, keep], got keep = " +
+                     std::to_string(keep) + ", recent = " + std::to_string(recent));
+        return -1;
+    }
+    const int64_t B = c->B, Hkv = c->Hkv, max_len = *std::max_element(c->len.begin(), c->len.end());
+    if (B * Hkv > 65535) {
+        gt_set_error(who + "batch * n_head_kv must be at most 65535");
+        return -1;
+    }
+    if (!weights && !c->sums) {
+        gt_set_error(who + "no attention weights have been accumulated (kv_cache_attention_accumulate), and none are given");
+        return -1;
+    }
+    if (weights && (weights->ndim != 3 || weights->shape[0] != B || weights->shape[1] != Hkv || weights->shape[2] < max_len)) {
+        gt_set_error(who + "weights must be (B = " + std::to_string(B) + ", Hkv = " + std::to_string(Hkv) +
+                     ", a weight for each of the " + std::to_string(max_len) + " tokens)");
+        return -1;
+    }
+    if (weights && !gt_is_float(weights->dtype)) {
+        gt_set_error(who + "weights must be a float tensor, got " + gt_dtype_name(weights->dtype));
+        return -1;
+    }
+    if (!gt_device_ok(c->dev)) return -1;
+    Temps tmp;
+    const gt_tensor *w = weights ? weights : c->sums;
+    if (w->device_type != GT_DEV_CUDA || w->device_index != c->dev || w->dtype != GT_F32) {
+        w = tmp.keep(gt_to_device_dense(w, c->dev, GT_F32));
+        if (!w) return -1;
+    }
+    const int64_t ksh[3] = {B, Hkv, keep}, lsh[1] = {B};
+    gt_tensor *kept = gt_new_tensor(3, ksh, GT_I64, GT_DEV_CUDA, c->dev);
+    if (!kept) return -1;
+    gt_tensor *owned = kept_out ? nullptr : tmp.keep(kept);
+    (void)owned;
+    const int32_t *len = (const int32_t *)gt_data(c->len_dev);
+    const int64_t *places = (const int64_t *)gt_data(kept);
+    bool ok = gt_hip_check(gt_launch_kv_select((const float *)gt_data(w), w->strides, len, (int64_t *)gt_data(kept), B, Hkv, keep, recent,
+                                               gt_stream()),
+                           "kv cache select kernel");
+    if (ok && max_len > keep) {
+        gt_tensor *count = tmp.keep(gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev));
+        // positions, which lengths no longer tell
+        if (!c->seen_dev) {
+            gt_tensor *a = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev), *b = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev);
+            ok = a && b && gt_hip_check(gt_launch_kv_advance(len, (int32_t *)gt_data(a), 0, B, gt_stream()), "kv cache positions kernel");
+            if (ok) {
+                c->seen_dev = a;
+                c->seen_next = b;
+            } else {
+                gt_tensor_free(a);
+                gt_tensor_free(b);
+            }
+        }
+        ok = ok && count &&
+             gt_hip_check(gt_launch_kv_evict_lengths(len, (int32_t *)gt_data(c->len_next), (int32_t *)gt_data(count), keep, B, gt_stream()),
+                          "kv cache lengths kernel");
+        gt_kv_moved moved[3];
+        int n = 0, zeroed = -1;
+        auto move = [&](gt_tensor *rows, int64_t row_bytes) {
+            const int64_t sh[1] = {B * Hkv * keep * row_bytes};
+            gt_tensor *t = tmp.keep(gt_new_tensor(1, sh, GT_U8, GT_DEV_CUDA, c->dev));
+            if (t) moved[n++] = {gt_data(rows), gt_data(t), row_bytes};
+            return t != nullptr;
+        };
+        if (ok && c->block) {
+            // the kept tokens' values, quantized again in their new blocks (exactly, where the scale stays)
+            const gt_kv_blocks blocks = kv_blocks_of(c);
+            const int64_t sh[4] = {B, Hkv, keep, c->D};
+            gt_tensor *kv[2];
+            for (gt_tensor *&t : kv) ok = ok && (t = tmp.keep(gt_new_tensor(4, sh, GT_F32, GT_DEV_CUDA, c->dev)));
+            ok = ok && gt_hip_check(gt_launch_kv_blocks_read(blocks, len, places, keep, gt_data(kv[0]), gt_data(kv[1]), GT_F32, gt_stream()),
+                                    "kv cache block read kernel");
+            if (ok) {
+                const void *data[2] = {gt_data(kv[0]), gt_data(kv[1])};
+                const int64_t *strides[2] = {kv[0]->strides, kv[1]->strides};
+                ok = gt_hip_check(gt_launch_kv_blocks_append(blocks, data, GT_F32, strides, nullptr, (const int32_t *)gt_data(count),
+                                                             nullptr, 0, keep / c->block, gt_stream()),
+                                  "kv cache block append kernel");
+            }
+        } else if (ok) {
+            const int64_t rb = (int64_t)gt_dtype_nbytes(c->dtype, c->D);
+            ok = move(c->k, rb) && move(c->v, rb);
+        }
+        if (ok && c->sums) {
+            zeroed = n;
+            ok = move(c->sums, sizeof(float));
+        }
+        ok = ok && gt_hip_check(gt_launch_kv_move(moved, n, zeroed, places, len, B, Hkv, keep, max_len, c->cap, gt_stream()),
+                                "kv cache move kernel");
+        if (ok) {
+            std::swap(c->len_dev, c->len_next);
+            for (auto &x : c->len) x = (int32_t)std::min<int64_t>(x, keep);
+        }
+    }
+    if (!ok) {
+        if (kept_out) gt_tensor_free(kept);
+        return -1;
+    }
+    if (kept_out) *kept_out = kept;
+    return 0;
+}
+
+int kv_read(gt_kv_cache *c, int dtype, gt_tensor **k, gt_tensor **v) {
+    const std::string who = "kv_cache_read: ";
+    if (!c || !k || !v) {
+        gt_set_error(who + "NULL argument");
+        return -1;
+    }
+    *k = *v = nullptr;
+    if (dtype != GT_F32 && dtype != GT_F16 && dtype != GT_BF16) {
+        gt_set_error(who + "dtype must be float32, float16 or bfloat16, got " + gt_dtype_name(dtype));
+        return -1;
+    }
+    if (!gt_device_ok(c->dev)) return -1;
+    const int64_t rows = *std::max_element(c->len.begin(), c->len.end()), sh[4] = {c->B, c->Hkv, rows, c->D};
+    gt_tensor *a = gt_new_tensor(4, sh, dtype, GT_DEV_CUDA, c->dev), *b = a ? gt_new_tensor(4, sh, dtype, GT_DEV_CUDA, c->dev) : nullptr;
+    const int32_t *len = (const int32_t *)gt_data(c->len_dev);
+    bool ok = a && b;
+    if (ok && rows > 0)
+        ok = gt_hip_check(c->block ? gt_launch_kv_blocks_read(kv_blocks_of(c), len, nullptr, rows, gt_data(a), gt_data(b), dtype, gt_stream())
+                                   : gt_launch_kv_rows_read(gt_data(c->k), gt_data(c->v), c->dtype, len, gt_data(a), gt_data(b), dtype,
+                                                            c->B, c->Hkv, rows, c->D, c->cap, gt_stream()),
+                          "kv cache read kernel");
+    if (!ok) {
+        gt_tensor_free(a);
+        gt_tensor_free(b);
+        return -1;
+    }
+    *k = a;
+    *v = b;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal) {
+    LaunchScope scope;
+    return kv_attention(c, q, scale, is_causal, nullptr);
+}
+
+extern "C" gt_tensor *gt_kv_cache_attention_accumulate(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal,
+                                                       float keep_factor) {
+    return guarded((gt_tensor *)nullptr, [&] {
+        LaunchScope scope;
+        return kv_attention_accumulate(c, q, scale, is_causal, keep_factor);
+    });
+}
+
+extern "C" gt_tensor *gt_kv_cache_weights(gt_kv_cache *c) {
+    return guarded((gt_tensor *)nullptr, [&]() -> gt_tensor * {
+        if (!c) {
+            gt_set_error("kv_cache_weights: NULL cache");
+            return nullptr;
+        }
+        if (!gt_device_ok(c->dev) || !kv_sums(c)) return nullptr;
+        return new gt_tensor(*c->sums);
+    });
+}
+
+extern "C" int gt_kv_cache_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weights, gt_tensor **kept) {
+    return guarded(-1, [&] { return kv_evict(c, keep, recent, weights, kept); });
+}
+
+extern "C" int gt_kv_cache_read(gt_kv_cache *c, int dtype, gt_tensor **k, gt_tensor **v) {
+    return guarded(-1, [&] { return kv_read(c, dtype, k, v); });
+}
+
+extern "C" int gt_kv_cache_append_rope_axes(gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int64_t pos_offset,
+                                            const gt_tensor *pos, int n_axes, const int *sections, int interleaved, int n_dims,
+                                            int mode, double freq_base, double freq_scale) {
+    return guarded(-1, [&] {
+        const char *who = "kv_cache_append_rope_axes";
+        if (!c) {
+            gt_set_error(std::string(who) + ": NULL cache");
+            return -1;
+        }
+        if (!kv_check_rows(who, c, k, "k") || !kv_check_rows(who, c, v, "v")) return -1;
+        Temps tmp;
+        if (k->dtype == GT_Q8_0 && !(k = tmp.keep(gt_dequantize(k, GT_F32)))) return -1;
+        const gt_tensor *turned = tmp.keep(gt_rope_axes(k, pos, n_axes, sections, interleaved, n_dims, mode, freq_base, freq_scale));
+        return turned ? kv_append(who, c, turned, v, pos_offset, nullptr) : -1;
+    });
 }

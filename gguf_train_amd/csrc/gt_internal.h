@@ -167,6 +167,84 @@ bool gt_rope_inline(int64_t numel, int64_t D);
 hipError_t gt_launch_rope(const void *x, int dtype, const int64_t *strides, void *y, const void *table,
                           int64_t table_b_stride, int64_t B, int64_t H, int64_t S, int64_t D, int n_dims, int mode,
                           hipStream_t stream, const gt_rope_angles *angles = nullptr);
+// The 8-bit block cache (kv_blocks.h): [0] keys, [1] values.
+struct gt_kv_blocks {
+    void *codes[2];
+    float *scales[2], *tail[2];
+    int64_t B, Hkv, D, units;
+    int N, Dp;
+    bool e4m3;
+};
+// Appends count[b] (null: T) rows of src[0] and src[1] (B, Hkv, T, D; float32, float16 or bfloat16, element
+// strides) after the pos[b] (null: 0) tokens that each sequence holds, quantizing the blocks that become
+// full, at most `blocks` of a sequence; pos_next[b] (null: not) becomes the tokens held afterwards.
+hipError_t gt_launch_kv_blocks_append(const gt_kv_blocks &c, const void *const *src, int src_dtype,
+                                      const int64_t *const *strides, const int32_t *pos, const int32_t *count,
+                                      int32_t *pos_next, int64_t T, int64_t blocks, hipStream_t s);
+// The values of tokens 0 .. rows - 1, or kept[b, g, 0 .. rows - 1], as dense (B, Hkv, rows, D) float32, float16
+// or bfloat16; zeros for tokens that are not held.
+hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, const int64_t *kept, int64_t rows,
+                                    void *k, void *v, int dtype, hipStream_t s);
+// Attention of few rows over the block cache (attn_kv_blocks.h): q (B, H, L, D) with contiguous dims, o dense of
+// q's dtype, lse (B, H, L) or null.  `note` describes the launch.
+constexpr int64_t kKvBlocksAttnRows = 128;
+struct gt_kv_blocks_attn {
+    const void *q;
+    void *o;
+    float *lse;
+    const int32_t *len;
+    int64_t q_strides[3], H, L, max_len;
+    int q_dtype, causal;
+    float scale;
+};
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype);
+hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note);
+// Sums of the attention weights of a cache's tokens (attn_key_weights.hip): sums (B, Hkv, cap) becomes keep *
+// sums + the weights' sums over the rows of q and the heads of a group, from the attention's lse.  The keys:
+// rows of k_dtype (B, Hkv, cap, D), or a block cache's.  D <= 256.
+struct gt_key_weights {
+    const void *q;
+    const void *k;
+    const gt_kv_blocks *blocks;  // or null
+    const float *lse;
+    const int32_t *len;
+    float *sums;
+    int64_t q_strides[3], B, H, Hkv, L, D, cap, max_len;
+    int q_dtype, k_dtype, causal;
+    float scale, keep;
+};
+hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s);
+// Eviction (kv_rows.hip).  Select: kept (B, Hkv, keep) = the tokens that stay, the `recent` last and those of the
+// largest weights w (element strides), in order; a sequence of at most `keep` tokens keeps them (-1 behind).
+hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int64_t *kept, int64_t B, int64_t Hkv,
+                               int64_t keep, int64_t recent, hipStream_t s);
+hipError_t gt_launch_kv_evict_lengths(const int32_t *len, int32_t *next, int32_t *count, int64_t keep, int64_t B, hipStream_t s);
+// Moves the kept rows of up to 3 tensors (B, Hkv, cap) together, through scratch (B, Hkv, keep); zeroed: the
+// one (4-byte rows) whose places left behind become zero, or -1.
+struct gt_kv_moved {
+    void *rows, *temp;
+    int64_t row_bytes;
+};
+hipError_t gt_launch_kv_move(const gt_kv_moved *t, int count, int zeroed, const int64_t *kept, const int32_t *len, int64_t B,
+                             int64_t Hkv, int64_t keep, int64_t max_len, int64_t cap, hipStream_t s);
+// The first `rows` tokens of a float or Q8_0 cache as dense (B, Hkv, rows, D) values; zeros past a length.
+hipError_t gt_launch_kv_rows_read(const void *k, const void *v, int dtype, const int32_t *len, void *ko, void *vo, int out_dtype,
+                                  int64_t B, int64_t Hkv, int64_t rows, int64_t D, int64_t cap, hipStream_t s);
+// RoPE with several axes (gt_rope_axes.hip): x (B, H, S, D) of a float dtype, any strides, into the dense y of
+// the same dtype; pos (axes, B, S) int32, int64, float32 or float64.  Head sizes up to kRopeAxesMaxDim (a
+// row's angles are kept in LDS).
+constexpr int64_t kRopeAxesMaxDim = 4096;
+struct gt_rope_axes_args {
+    const void *x;
+    void *y;
+    const void *pos;
+    int dtype, pos_dtype;
+    int64_t x_strides[4], pos_strides[3];
+    int64_t B, H, S, D;
+    int n_axes, sections[4], interleaved, n_dims, mode, backward;
+    double freq_base, freq_scale;
+};
+hipError_t gt_launch_rope_axes(const gt_rope_axes_args &r, hipStream_t s);
 // ---- RoPE argument checks (gt_rope_ops.cpp) ----------------------------------------------------
 // mode 0/2, even n_dims in [2, head_dim], positive finite freq_base, finite freq_scale; the
 // reference's messages prefixed with `who`.

@@ -154,3 +154,139 @@ extern "C" gt_tensor *gt_rope_backward(const gt_tensor *grad_out, const gt_tenso
     if (!rope_check(grad_out, pos, n_dims, mode, freq_base, freq_scale, L)) return nullptr;
     return rope_run(grad_out, pos, L, n_dims, mode, freq_base, freq_scale, true);
 }
+
+// ---- several axes ----------------------------------------------------------------------------
+// The reference refuses the modes with per-section positions (csrc/gt_ops_nn.cpp:2311-2349); these are
+// entry points of their own.
+
+namespace {
+
+bool axes_check(const char *who, const gt_tensor *x, const gt_tensor *pos, int n_axes, const int *sections,
+                int interleaved, int n_dims, int mode, double freq_base, double freq_scale, gt_rope_axes_args &r) {
+    const std::string w = std::string(who) + ": ";
+    if (!x || !pos || !sections) {
+        gt_set_error(w + "x, pos and sections are required");
+        return false;
+    }
+    if (x->ndim < 3 || x->ndim > 4) {
+        gt_set_error(w + "expected x of shape (batch, heads, seq_len, head_dim) or (heads, seq_len, head_dim), got " +
+                     shape_str(x));
+        return false;
+    }
+    if (!gt_is_float(x->dtype)) {
+        gt_set_error(w + "x must be a floating point tensor");
+        return false;
+    }
+    const int o = x->ndim == 4 ? 1 : 0;
+    r.B = o ? x->shape[0] : 1;
+    r.H = x->shape[o];
+    r.S = x->shape[o + 1];
+    r.D = x->shape[o + 2];
+    for (int i = 0; i < 4; ++i) r.x_strides[i] = i + o - 1 < 0 ? 0 : x->strides[i + o - 1];
+    // (the check takes floats, which a finite double need not fit)
+    const bool freq_ok = freq_base > 0.0 && std::isfinite(freq_base) && std::isfinite(freq_scale);
+    if (!gt_rope_check_args(who, r.D, n_dims, mode, freq_ok ? 1.0f : -1.0f, 1.0f)) return false;
+    if (r.D > kRopeAxesMaxDim) {
+        gt_set_error(w + "head dimensions above " + std::to_string(kRopeAxesMaxDim) + " are not supported, got " +
+                     std::to_string(r.D));
+        return false;
+    }
+    if (n_axes < 1 || n_axes > 4) {
+        gt_set_error(w + "1 to 4 axes are supported, got " + std::to_string(n_axes));
+        return false;
+    }
+    int64_t sum = 0;
+    std::string list;
+    for (int i = 0; i < n_axes; ++i) {
+        list += (i ? ", " : "") + std::to_string(sections[i]);
+        sum = sections[i] < 0 ? -(1LL << 40) : sum + sections[i];
+        r.sections[i] = sections[i];
+    }
+    if (sum != n_dims / 2) {
+        gt_set_error(w + "sections [" + list + "] must be pairs of each axis, n_dims / 2 = " + std::to_string(n_dims / 2) +
+                     " in all");
+        return false;
+    }
+    for (int i = 1; interleaved && i < n_axes; ++i) {
+        if (sections[i] > 0 && (int64_t)n_axes * (sections[i] - 1) + i >= n_dims / 2) {
+            gt_set_error(w + "interleaved sections [" + list + "]: axis " + std::to_string(i) + " does not fit, its pairs are " +
+                         "every " + std::to_string(n_axes) + "th of " + std::to_string(n_dims / 2));
+            return false;
+        }
+    }
+    if (pos->ndim < 2 || pos->ndim > 3 || pos->shape[0] != n_axes || pos->shape[pos->ndim - 1] < r.S ||
+        (pos->ndim == 3 && pos->shape[1] != r.B && pos->shape[1] != 1)) {
+        gt_set_error(w + "pos must be of shape (axes, seq_len) or (axes, batch, seq_len), axes = " + std::to_string(n_axes) +
+                     ", batch = " + std::to_string(r.B) + ", with a position for each of the " + std::to_string(r.S) +
+                     " sequence elements, got " + shape_str(pos));
+        return false;
+    }
+    if (gt_is_quantized(pos->dtype) || pos->dtype == GT_BOOL) {
+        gt_set_error(w + "pos must hold integer or float positions, got " + gt_dtype_name(pos->dtype));
+        return false;
+    }
+    r.n_axes = n_axes;
+    r.interleaved = interleaved ? 1 : 0;
+    r.n_dims = n_dims;
+    r.mode = mode;
+    r.freq_base = freq_base;
+    r.freq_scale = freq_scale;
+    return true;
+}
+
+gt_tensor *axes_run(const char *who, const gt_tensor *x, const gt_tensor *pos, int n_axes, const int *sections,
+                    int interleaved, int n_dims, int mode, double freq_base, double freq_scale, bool backward) {
+    gt_rope_axes_args r{};
+    if (!axes_check(who, x, pos, n_axes, sections, interleaved, n_dims, mode, freq_base, freq_scale, r)) return nullptr;
+    if (x->numel == 0) return gt_tensor_empty(x->ndim, x->shape, x->dtype, x->device_type, x->device_index);
+    const int dev = x->device_type == GT_DEV_CUDA ? x->device_index : 0;
+    if (!gt_device_ok(dev)) return nullptr;
+    gt_tensor *xs_owned = nullptr, *ps_owned = nullptr;
+    const gt_tensor *xs = x, *ps = pos;
+    if (x->device_type != GT_DEV_CUDA) {
+        xs = xs_owned = gt_to_device_dense(x, dev, -1);
+        r.x_strides[3] = 1;
+        r.x_strides[2] = r.D;
+        r.x_strides[1] = r.S * r.D;
+        r.x_strides[0] = x->ndim == 4 ? r.H * r.S * r.D : 0;
+    }
+    // int32, int64, float32 and float64 positions are read where they are; others as float64, exactly
+    const bool read = pos->dtype == GT_I32 || pos->dtype == GT_I64 || pos->dtype == GT_F32 || pos->dtype == GT_F64;
+    if (xs && (!read || pos->device_type != GT_DEV_CUDA || pos->device_index != dev))
+        ps = ps_owned = gt_to_device_dense(pos, dev, read ? -1 : GT_F64);
+    gt_tensor *out = xs && ps ? gt_new_tensor(x->ndim, x->shape, x->dtype, GT_DEV_CUDA, dev) : nullptr;
+    bool ok = out != nullptr;
+    if (ok) {
+        r.x = gt_data(xs);
+        r.y = gt_data(out);
+        r.pos = gt_data(ps);
+        r.dtype = x->dtype;
+        r.pos_dtype = ps->dtype;
+        r.pos_strides[0] = ps->strides[0];
+        r.pos_strides[1] = ps->ndim == 3 && ps->shape[1] > 1 ? ps->strides[1] : 0;
+        r.pos_strides[2] = ps->strides[ps->ndim - 1];
+        r.backward = backward;
+        ok = gt_hip_check(gt_launch_rope_axes(r, gt_stream()), "rope_axes kernel");
+    }
+    gt_tensor_free(xs_owned);
+    gt_tensor_free(ps_owned);
+    if (!ok) {
+        gt_tensor_free(out);
+        return nullptr;
+    }
+    return gt_deliver(out, x->device_type != GT_DEV_CUDA);
+}
+
+}  // namespace
+
+extern "C" gt_tensor *gt_rope_axes(const gt_tensor *x, const gt_tensor *pos, int n_axes, const int *sections,
+                                   int interleaved, int n_dims, int mode, double freq_base, double freq_scale) {
+    return axes_run("rope_axes", x, pos, n_axes, sections, interleaved, n_dims, mode, freq_base, freq_scale, false);
+}
+
+extern "C" gt_tensor *gt_rope_axes_backward(const gt_tensor *grad_out, const gt_tensor *pos, int n_axes,
+                                            const int *sections, int interleaved, int n_dims, int mode,
+                                            double freq_base, double freq_scale) {
+    return axes_run("rope_axes_backward", grad_out, pos, n_axes, sections, interleaved, n_dims, mode, freq_base,
+                    freq_scale, true);
+}

@@ -215,6 +215,7 @@ const char *gt_dtype_name(int dtype) {
         case GT_BOOL: return "bool";
         case GT_C64: return "complex64";
         case GT_C128: return "complex128";
+        case GT_F8E4M3: return "float8_e4m3";
         case GT_Q8_0: return "q8_0";
         default: return "unknown";
     }

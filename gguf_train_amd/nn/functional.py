@@ -23,7 +23,7 @@ import math
 import torch
 
 from .._bridge import QuantizedTensor
-from .._functions import FlashAttentionDropoutFn, FlashAttentionFn, RoPEFn, draw_dropout_seed
+from .._functions import FlashAttentionDropoutFn, FlashAttentionFn, RoPEAxesFn, RoPEFn, draw_dropout_seed
 from .. import _ops
 
 
@@ -91,3 +91,20 @@ def rope(input, positions, n_dims: int | None = None, mode: int = 0, n_ctx_orig:
     seq_len are used); n_dims defaults to head_dim; mode 0 NORMAL, 2 NeoX."""
     nd = input.shape[-1] if n_dims is None else int(n_dims)
     return RoPEFn.apply(input, positions, nd, int(mode), int(n_ctx_orig), float(freq_base), float(freq_scale))
+
+
+def rope_axes(input, positions, sections, n_dims: int | None = None, mode: int = 2, interleaved: bool = False,
+              freq_base: float = 10000.0, freq_scale: float = 1.0):
+    """Rotary position embedding of tokens with positions on several axes, e.g. (time, height, width) of the
+    patches of an image or a video, text having the same position on each.
+
+    input (batch, heads, seq_len, head_dim) or (heads, seq_len, head_dim); positions (axes, seq_len) or (axes,
+    batch, seq_len), integer or float (the first seq_len are used); sections: the number of pairs that turn
+    with each axis, n_dims / 2 in all (n_dims defaults to head_dim).  Pair i has the frequency that `rope` gives
+    it, freq_base^(-2i/n_dims).  interleaved False: the sections follow each other along the pairs; True: the
+    axes take turns, pair i going to axis i % axes until that axis has its section's pairs, to the first axis
+    afterwards.  mode 2 NeoX (pairs (i, i + n_dims/2)), 0 NORMAL.  Angles are formed in float64, so far positions
+    keep their precision; differentiable in input."""
+    nd = input.shape[-1] if n_dims is None else int(n_dims)
+    return RoPEAxesFn.apply(input, positions, tuple(int(n) for n in sections), nd, int(mode), bool(interleaved),
+                            float(freq_base), float(freq_scale))

@@ -53,6 +53,9 @@ enum gt_dtype {
     GT_BOOL = 9,
     GT_C64 = 10,
     GT_C128 = 11,
+    /* No counterpart in the reference: float8 e4m3 (OCP, no infinities), the codes of a block cache
+     * (gt_kv_cache_create_blocks); no tensor has it. */
+    GT_F8E4M3 = 12,
     GT_Q_BASE = 100
 };
 /* GGUF Q8_0: blocks of 32 values, {fp16 d, int8 qs[32]} = 34 bytes (ggml type 8;
@@ -294,6 +297,22 @@ GT_API gt_tensor *gt_flash_attention_rope(const gt_tensor *q, const gt_tensor *k
                                           const gt_tensor *mask, float scale, int is_causal, const gt_tensor *pos,
                                           int n_dims, int mode, float freq_base, float freq_scale);
 
+/* No counterpart in the reference, whose gt_rope refuses the modes with positions of several axes.  RoPE
+ * of tokens that have n_axes (1 to 4) positions each, e.g. time, height and width: x as gt_rope; pos (axes,
+ * seq_len) or (axes, batch, seq_len; a batch of 1 is shared), any integer or float dtype and strides, with
+ * at least seq_len positions, fractions kept.  sections[a]: how many of the n_dims / 2 pairs turn with axis a
+ * (they add up to n_dims / 2).  interleaved 0: the first sections[0] pairs with axis 0, the next with axis 1
+ * and so on; otherwise pair i with axis i % n_axes while i / n_axes < sections of that axis, else with axis 0.
+ * mode 0 (pairs (2i, 2i+1)) or 2 (pairs (i, i + n_dims/2)); elements from n_dims on pass through.  Angle of
+ * pair i: freq_scale * pos * freq_base^(-2i/n_dims), formed in float64 (gt_rope forms it in float32); rotation
+ * in float32 (float64 x: float64), rounded once.  head_dim up to 4096.  The backward is the inverse rotation.
+ * Result: a new dense tensor of x's shape, dtype and device. */
+GT_API gt_tensor *gt_rope_axes(const gt_tensor *x, const gt_tensor *pos, int n_axes, const int *sections,
+                               int interleaved, int n_dims, int mode, double freq_base, double freq_scale);
+GT_API gt_tensor *gt_rope_axes_backward(const gt_tensor *grad_out, const gt_tensor *pos, int n_axes,
+                                        const int *sections, int interleaved, int n_dims, int mode,
+                                        double freq_base, double freq_scale);
+
 /* ---- GGUF Q8_0 ------------------------------------------------------------------------ */
 
 /* csrc/gguf_train.h:381 (gt_tensor_to_dtype, csrc/gt_core.cpp:784-847): quantizes rows of
@@ -380,6 +399,50 @@ GT_API int gt_kv_cache_append_rope(gt_kv_cache *c, const gt_tensor *k, const gt_
  * cached token.  scale <= 0 means 1/sqrt(head_dim).  Output (batch, H, L, head_dim), dtype
  * and device of q. */
 GT_API gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal);
+
+/* The rest has no counterpart in the reference.
+ *
+ * A block cache: keys and values in 8 bits, code x scale with one scale for each block of block_tokens (32, 64
+ * or 128) tokens of a sequence and kv head, for K and V apart.  dtype GT_I8 (codes of -127 .. 127) or GT_F8E4M3.
+ * The scale is the smallest power of two (2^-126 at least) that brings the block's largest magnitude within 127
+ * or 448; a value is rounded to the nearest code, ties to even.  A sequence's tokens after its last whole block
+ * are held in float32, and are quantized when their block is full: what the cache holds does not depend on how
+ * the tokens were appended.  A block with an infinity or NaN reads as NaN.  head_dim up to 256 (storage is
+ * padded to 64, 128 or 256), batch * n_head_kv up to 65535.  The gt_kv_cache_* entry points take it like any
+ * other cache, but for gt_kv_cache_keys / values, which fail (gt_kv_cache_read gives the values); float64 rows
+ * are rounded to float32.  Attention is computed on the values: float32, float16 and bfloat16 queries of up to
+ * 128 rows per kv head (H / n_head_kv * L) straight from the codes; other calls read the values into a
+ * temporary first, in the queries' dtype if every token was appended in it, else in float32. */
+GT_API gt_kv_cache *gt_kv_cache_create_blocks(int64_t batch, int64_t n_head_kv, int64_t capacity, int64_t head_dim,
+                                              int dtype, int block_tokens, int device_index);
+/* The values a cache of any dtype stands for: new device tensors (batch, n_head_kv, longest length, head_dim)
+ * of dtype GT_F32, GT_F16 (finite values stay finite) or GT_BF16; zeros past a sequence's length. */
+GT_API int gt_kv_cache_read(gt_kv_cache *c, int dtype, gt_tensor **k, gt_tensor **v);
+/* gt_kv_cache_append with the keys rotated as gt_rope_axes rotates them, at the positions given (axes, T) or
+ * (axes, batch, T): the cache then holds what gt_rope_axes followed by gt_kv_cache_append would store. */
+GT_API int gt_kv_cache_append_rope_axes(gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int64_t pos_offset,
+                                        const gt_tensor *pos, int n_axes, const int *sections, int interleaved,
+                                        int n_dims, int mode, double freq_base, double freq_scale);
+/* gt_kv_cache_attention that also counts the attention weight of each token held: for the call's softmax
+ * weights p, a[b, g, t] becomes keep_factor * a[b, g, t] + the sum of p[b, h, l, t] over the query heads h of kv
+ * head g and the rows l, in float32 (keep_factor in [0, 1]: 1 adds to what was counted so far, 0 starts anew).
+ * q float32, float16 or bfloat16 with at least one row, head_dim up to 256. */
+GT_API gt_tensor *gt_kv_cache_attention_accumulate(gt_kv_cache *c, const gt_tensor *q, float scale, int is_causal,
+                                                   float keep_factor);
+/* A new handle sharing the accumulated weights (batch, n_head_kv, capacity) float32; zeros past a sequence's
+ * length and for tokens appended since.  gt_kv_cache_clear clears a sequence's. */
+GT_API gt_tensor *gt_kv_cache_weights(gt_kv_cache *c);
+/* Cuts every sequence that holds more than `keep` tokens to `keep`: for each kv head apart, its `recent` last
+ * tokens and the keep - recent others of the largest weights (the earliest of equal ones; a NaN counts as the
+ * largest), in their order.  weights: float (batch, n_head_kv, at least the longest length), NULL for the
+ * accumulated ones; those of the tokens that stay, stay with them.  A block cache's tokens are quantized again
+ * in their new blocks (exactly, unless their scale grows).  kept (NULL: not wanted) receives a new device tensor
+ * (batch, n_head_kv, keep) int64, the index each kept token had, -1 past a shorter sequence's length.
+ * Positions go on from what was appended, not from the length: gt_kv_cache_position, pos_offset and the
+ * angles of gt_kv_cache_append_rope count evicted tokens.  Keys are kept as they were appended (rotated). */
+GT_API int gt_kv_cache_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weights, gt_tensor **kept);
+/* The position of sequence `seq`'s next token: the tokens appended to it since it was empty (-1 on error). */
+GT_API int64_t gt_kv_cache_position(const gt_kv_cache *c, int64_t seq);
 
 #ifdef __cplusplus
 }
