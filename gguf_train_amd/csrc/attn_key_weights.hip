@@ -15,19 +15,22 @@
 #include "attn_kv_blocks.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace {
 
 using namespace gtkvb;
 
-enum Source { kInt8, kE4m3, kF16, kBf16, kF32, kQ8 };
+enum Source { kInt8, kE4m3, kF16, kBf16, kF32, kQ8, kAny };  // kAny: float rows not in whole aligned pieces of 16 dims
 
 struct Args {
     const void *q;
     int64_t q_sb, q_sh, q_sl;
     const char *k;  // rows (B, Hkv, cap); the codes of a block cache
     int64_t row_bytes, cap;
-    const float *ks, *kt;  // a block cache's scales and tail
+    const float *ks;       // a block cache's scales, and its tail's operands and scales
+    const _Float16 *kt;
+    const float *kts;
     int N;
     int64_t units;
     const float *lse;
@@ -36,37 +39,79 @@ struct Args {
     float *parts;  // (splits, B, Hkv, cap), or null: one split writes sums
     float keep;
     float scale;
-    int causal, q_vec;
+    int causal, q_vec, k_dtype;
     int H, Hkv, L, D;
     int col_tiles, span;  // columns of 16 rows in all, and per split
 };
 
-__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kF32>) { return ((const float *)row)[d]; }
-__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kF16>) { return (float)((const _Float16 *)row)[d]; }
-__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kBf16>) { return (float)((const __bf16 *)row)[d]; }
-__device__ inline float key_value(const char *row, int d, std::integral_constant<int, kQ8>) {
-    const uint8_t *blk = (const uint8_t *)row + (d >> 5) * 34;
-    return (float)*(const _Float16 *)blk * (float)*(const int8_t *)(blk + 2 + (d & 31));
-}
-
-// The A operands of key `t` (this lane's, of 16; zeros when it is not there) and its scale; lanes g hold dims
-// 16 (4i + g) .. +15.
-template <int KIND, int NI>
-__device__ inline float key_operands(const char *row, bool there, int D, int g, half8 (*hi)[2], half8 (*lo)[2]) {
-    float x[NI][16];
-    float amax = 0.0f;
-    bool odd = false;
+// Dims d0 .. d0 + 15 of a row of keys as they lie in memory, from an address inside the row whatever d0 (no branch
+// around a load: all of a wavefront's are in flight together), and then as values.
+template <int KIND>
+struct KeyDims {
+    typedef std::conditional_t<KIND == kF32, float, std::conditional_t<KIND == kBf16, __bf16, _Float16>> T;
+    gtvec::Dims16<T> piece;
+    __device__ void load(const char *row, int d0, int, int D) { piece.load((const T *)row + (d0 < D ? d0 : 0)); }
+    __device__ void values(int d0, int D, float *x) const {  // zeros from D on
 #pragma unroll
-    for (int i = 0; i < NI; ++i)
+        for (int e = 0; e < 16; ++e) x[e] = d0 < D ? piece.get(e) : 0.0f;
+    }
+};
+template <>
+struct KeyDims<kQ8> {  // half a block of 32: its scale, and 16 codes in steps of 2 bytes
+    uint16_t w[8], scale;
+    __device__ void load(const char *row, int d0, int, int D) {
+        const int d = d0 < D ? d0 : 0;
+        const uint8_t *blk = (const uint8_t *)row + (d >> 5) * 34;
+        scale = *(const uint16_t *)blk;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = *(const uint16_t *)(blk + 2 + (d & 31) + 2 * e);
+    }
+    __device__ void values(int d0, int D, float *x) const {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            x[e] = d0 < D ? (float)__builtin_bit_cast(_Float16, scale) * (float)(int8_t)(w[e / 2] >> (8 * (e & 1))) : 0.0f;
+    }
+};
+template <>
+struct KeyDims<kAny> {
+    float v[16];
+    __device__ void load(const char *row, int d0, int dtype, int D) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int d = 16 * (4 * i + g) + e;
-            x[i][e] = there && d < D ? key_value(row, d, std::integral_constant<int, KIND>{}) : 0.0f;
-            amax = fmaxf(amax, fabsf(x[i][e]));
-            odd = odd || !(fabsf(x[i][e]) < INFINITY);
+            const int d = min(d0 + e, D - 1);
+            v[e] = dtype == GT_F32 ? ((const float *)row)[d] : dtype == GT_F16 ? (float)((const _Float16 *)row)[d] : (float)((const __bf16 *)row)[d];
         }
-    amax = max_g(odd ? INFINITY : amax);
-    odd = amax == INFINITY;  // (an infinity or NaN: the key's scores are NaN, and no other key's)
+    }
+    __device__ void values(int d0, int D, float *x) const {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = d0 + e < D ? v[e] : 0.0f;
+    }
+};
+
+// The A operands of a key row of which this lane holds dims 16 (4i + g) .. +15, and the row's scale (the same in the
+// four lanes).
+template <int KIND, int NI>
+__device__ inline float key_operands(const KeyDims<KIND> *raw, int D, int g, half8 (*hi)[2], half8 (*lo)[2]) {
+    if constexpr (KIND == kF16) {  // its own operand
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const u32x4 w = raw[i].piece.w[j];
+                hi[i][j] = __builtin_bit_cast(half8, 16 * (4 * i + g) < D ? w : u32x4{0u, 0u, 0u, 0u});
+            }
+        return 1.0f;
+    }
+    float x[NI][16];
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        raw[i].values(16 * (4 * i + g), D, x[i]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[i][e]) < INFINITY ? fabsf(x[i][e]) : INFINITY);
+    }
+    amax = max_g(amax);
+    const bool odd = amax == INFINITY;  // (an infinity or NaN: the key's scores are NaN, and no other key's)
     const int e2 = exponent_of(amax);
     const float inv = pow2(-e2);
 #pragma unroll
@@ -83,7 +128,7 @@ __device__ inline float key_operands(const char *row, bool there, int D, int g, 
 template <typename QT, int SRC, int NI, int TW>
 __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
     constexpr bool CODES = SRC == kInt8 || SRC == kE4m3;
-    constexpr bool KLO = CODES || SRC == kF32 || SRC == kQ8;  // keys may need lo operands (a tail's do)
+    constexpr bool KLO = CODES || SRC == kF32 || SRC == kQ8 || SRC == kAny;  // keys may need lo operands (a tail's do)
     constexpr bool QLO = __is_same(QT, float);
     constexpr int Dp = 64 * NI;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -96,9 +141,17 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
     half8 kh[TW][NI][2], kl[TW][NI][2];
     float ksc[TW][4];
     bool lo_used = !CODES && KLO;
+    KeyDims<CODES ? kF32 : SRC> raw[CODES ? 1 : TW][NI];
+    if constexpr (!CODES) {
+#pragma unroll
+        for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)  // (tokens that are not there: the last one, left out below)
+                raw[kb][i].load(a.k + (bg * a.cap + min(k0 + 16 * kb + n, len - 1)) * a.row_bytes, 16 * (4 * i + g), a.k_dtype, a.D);
+    }
 #pragma unroll
     for (int kb = 0; kb < TW; ++kb) {
-        const int t0 = k0 + 16 * kb, t = t0 + n;
+        const int t0 = k0 + 16 * kb;
         if (CODES && t0 < full) {  // (a whole block is a multiple of 16 tokens)
             const uint8_t *p = (const uint8_t *)a.k + bg * a.units * kUnit * Dp + (int64_t)t0 * Dp + 16 * lane;
 #pragma unroll
@@ -113,15 +166,22 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
             const float s = a.ks[bg * (a.units * kUnit / a.N) + t0 / a.N];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = s;
+        } else if constexpr (CODES) {
+            lo_used = true;
+            const int room = max(a.N, kUnit), at = min(t0 - full, room - 16);  // (the last tiles may hold no token)
+            const _Float16 *p = a.kt + (bg * 2 * room + at) * Dp + 16 * lane;
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    kh[kb][i][j] = *(const half8 *)(p + 1024 * i + 8 * j);
+                    kl[kb][i][j] = *(const half8 *)(p + (int64_t)room * Dp + 1024 * i + 8 * j);
+                }
+            const f32x4 s = *(const f32x4 *)(a.kts + bg * room + at + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ksc[kb][i] = s[i];
         } else {
-            float s;
-            if constexpr (CODES) {
-                lo_used = true;
-                const int tt = t - full;
-                s = key_operands<kF32, NI>((const char *)(a.kt + (bg * a.N + tt) * a.D), t < len, a.D, g, kh[kb], kl[kb]);
-            } else {
-                s = key_operands<SRC, NI>(a.k + (bg * a.cap + t) * a.row_bytes, t < len, a.D, g, kh[kb], kl[kb]);
-            }
+            const float s = key_operands<SRC, NI>(raw[kb], a.D, g, kh[kb], kl[kb]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = __shfl(s, 4 * g + i, 64);
         }
@@ -206,7 +266,8 @@ const void *kernel_src(int src, int Dp) {
         case kF16: return kernel_d<QT, kF16>(Dp);
         case kBf16: return kernel_d<QT, kBf16>(Dp);
         case kF32: return kernel_d<QT, kF32>(Dp);
-        default: return kernel_d<QT, kQ8>(Dp);
+        case kQ8: return kernel_d<QT, kQ8>(Dp);
+        default: return kernel_d<QT, kAny>(Dp);
     }
 }
 
@@ -227,7 +288,7 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
     a.scale = r.scale;
     a.causal = r.causal;
     const int64_t per16 = r.q_dtype == GT_F32 ? 4 : 8;
-    a.q_vec = (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
+    a.q_vec = r.D % 16 == 0 && (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
     a.H = (int)r.H;
     a.Hkv = (int)r.Hkv;
     a.L = (int)r.L;
@@ -237,13 +298,16 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
         src = r.blocks->e4m3 ? kE4m3 : kInt8;
         a.k = (const char *)r.blocks->codes[0];
         a.ks = r.blocks->scales[0];
-        a.kt = r.blocks->tail[0];
+        a.kt = (const _Float16 *)r.blocks->ops[0];
+        a.kts = r.blocks->op_scales[0];
         a.N = r.blocks->N;
         a.units = r.blocks->units;
     } else {
         src = r.k_dtype == GT_F16 ? kF16 : r.k_dtype == GT_BF16 ? kBf16 : r.k_dtype == GT_F32 ? kF32 : kQ8;
         a.k = (const char *)r.k;
         a.row_bytes = r.k_dtype == GT_Q8_0 ? r.D / 32 * 34 : r.k_dtype == GT_F32 ? r.D * 4 : r.D * 2;
+        a.k_dtype = r.k_dtype;
+        if (src != kQ8 && (r.D % 16 != 0 || (uintptr_t)r.k % 16 != 0)) src = kAny;
     }
     const int Dp = padded_dim(r.D), keys = 16 * (Dp == 256 ? 2 : 4) * kWaves;
     const void *kernel = r.q_dtype == GT_F16   ? kernel_src<_Float16>(src, Dp)

@@ -11,8 +11,8 @@
 // running maximum and sum; they are joined once at the end, and the last split of a row group to finish joins
 // the splits (partials in uncached memory, as in decode_merge.h).
 //
-// Products on v_mfma_f32_16x16x32_f16, float32 sums.  Codes become float16 exactly: int8 by placing two bytes
-// under exponent bytes (1024 + 128 + code) and subtracting 1152, e4m3 by the hardware's conversion.
+// Products on v_mfma_f32_16x16x32_f16, float32 sums.  Codes become float16 exactly: int8 (kept as code + 128) by placing
+// two bytes under exponent bytes (1024 + 128 + code) and subtracting 1152, e4m3 by the hardware's conversion.
 // Score S^T = K.Q^T: float16 queries are their own operand; bfloat16 and float32 rows are scaled by a power of
 // two to a largest magnitude in [1, 2) and enter as one operand (bfloat16: exact, but for elements below 2^-14
 // of the largest, which keep 2^-25 of it) or as two, x = hi + lo (float32: off by 2^-25 of the largest).
@@ -20,21 +20,24 @@
 // what float16 loses below 2^-14 is small against the largest term, whatever the blocks' scales.  float16 and
 // bfloat16 results take p' rounded to float16 (2^-12 of each term), float32 results take hi + lo.
 //
-// The tail's float32 tokens are one or two more units: a key's row (K and V) is scaled by its own power of two
-// and split into hi + lo operands, which carry 22 bits.  A key with an infinity or NaN has codes of zero and a
-// NaN for a scale, which only the rows that see it meet.
+// The tail is one or two more units, of the operands that the append has left: a token's row (K and V) divided
+// by its own power of two, as float16 hi + lo, which carry 22 bits.  A token with an infinity or NaN has operands
+// of zero and a NaN for a scale, which only the rows that see it meet.  (Formed here, from the float32 tokens, they
+// took 30 us of a decode step, in loads one after the other.)
 #pragma once
 
 #include "attn_common.h"
 #include "gt_internal.h"
 #include "kv_blocks.h"
 #include "mfma_util.h"
+#include "vec_dims.h"
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <type_traits>
 
 namespace gtkvb {
 
@@ -54,10 +57,12 @@ struct AttnArgs {
     void *o;                   // dense (B, H, L, D) of q's type
     float *lse;                // (B, H, L) or null
     const uint8_t *k, *v;
-    const float *ks, *vs, *kt, *vt;  // scales and tails
+    const float *ks, *vs;  // scales
+    const _Float16 *kt, *vt;  // the tail's operands, hi then lo
+    const float *kts, *vts;   // and scales
     const int32_t *len;
     float scale;
-    int causal, q_vec;  // q_vec: query rows in aligned 16-byte pieces
+    int causal, q_vec;  // q_vec: query rows in aligned 16-byte pieces, D a multiple of 16
     int B, H, Hkv, L, D, N;
     int64_t units;  // of a slice
     int groups;     // row groups per kv head
@@ -84,6 +89,9 @@ __device__ inline int exponent_of(float a) {
     return min(max((int)(__float_as_uint(a) >> 23) - 127, -126), 126);
 }
 
+// The exponent of a scale (a power of two), NaN for a NaN.
+__device__ inline float exponent_bits(uint32_t b) { return (b >> 23 & 255) == 255 ? NAN : (float)((int)(b >> 23) - 127); }
+
 // Eight codes as float16.
 template <bool E4M3>
 __device__ inline half8 decode8(uint32_t w0, uint32_t w1) {
@@ -94,10 +102,8 @@ __device__ inline half8 decode8(uint32_t w0, uint32_t w1) {
         h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
         h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
     } else {
-        // bytes u = code + 128 under 0x64: 1024 + u
+        // bytes code + 128 under 0x64: 1024 + 128 + code
         const half2v off = {(_Float16)1152.0f, (_Float16)1152.0f};
-        w0 ^= 0x80808080u;
-        w1 ^= 0x80808080u;
         constexpr uint32_t k64 = 0x64646464u;
         h[0] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w0, 0x04010400u)) - off;
         h[1] = __builtin_bit_cast(half2v, (uint32_t)__builtin_amdgcn_perm(k64, w0, 0x04030402u)) - off;
@@ -127,28 +133,28 @@ template <typename QT, int NI>
 __device__ inline float load_query(const QT *row, int D, bool vec, int g, half8 (*hi)[2], half8 (*lo)[2]) {
     constexpr bool F16 = __is_same(QT, _Float16);
     float x[NI][16];
+    if (vec) {  // rows in aligned 16-byte pieces, D a multiple of 16
+        gtvec::Dims16<QT> raw[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) raw[i].load(row + (16 * (4 * i + g) < D ? 16 * (4 * i + g) : 0));
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[i][e] = 16 * (4 * i + g) < D ? raw[i].get(e) : 0.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = 16 * (4 * i + g) + e;
+                x[i][e] = d < D ? (float)row[d] : 0.0f;
+            }
+    }
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-        const int d0 = 16 * (4 * i + g);
-        if (vec && d0 + 16 <= D) {
-            struct alignas(16) P {
-                QT e[16 / sizeof(QT)];
-            };
-            constexpr int PER = 16 / sizeof(QT);
-#pragma unroll
-            for (int p = 0; p < 16 / PER; ++p) {
-                const P piece = *(const P *)(row + d0 + p * PER);
-#pragma unroll
-                for (int e = 0; e < PER; ++e) x[i][p * PER + e] = (float)piece.e[e];
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[i][e] = d0 + e < D ? (float)row[d0 + e] : 0.0f;
-        }
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(x[i][e]));
-    }
     int e2 = 0;
     if constexpr (!F16) e2 = exponent_of(max_g(amax));
     const float inv = F16 ? 1.0f : pow2(-e2);
@@ -159,53 +165,77 @@ __device__ inline float load_query(const QT *row, int D, bool vec, int g, half8 
     return pow2(e2);
 }
 
-// Joins the splits of rows row0 .. row0 + n - 1, one wavefront a row; uncached partials (see decode_merge.h).
+// Joins the splits of rows row0 .. row0 + n - 1; uncached partials (see decode_merge.h), each load a round trip
+// to the memory: the (max, sum) pairs of all rows first, into LDS, then every thread four dims of a row, eight
+// splits in flight.  lds: n * nsplit floats.
 template <typename TO, int NI>
-__device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n) {
-    constexpr int Dp = 64 * NI;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ns = a.nsplit;
-    for (int r = w; r < n; r += kWaves) {
-        const int64_t row = row0 + r;
-        const float *ml = a.part_ml + row * ns * 2, *po = a.part_o + row * ns * Dp + lane;
-        // (max, sum) of split `lane`; at most 64 splits
-        const float mi = lane < ns ? ml[2 * lane] : -INFINITY, li = lane < ns ? ml[2 * lane + 1] : 0.0f;
-        float M = mi, L;
-        for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-        const float wi = mi == -INFINITY && !(li != li) ? 0.0f : fast_exp2(mi - (M == -INFINITY ? 0.0f : M));
-        L = wi * li;
-        if (li != li) L = li;
-        for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
-        float acc[NI];
+__device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, float *lds) {
+    constexpr int Dp = 64 * NI, PIECES = Dp / 4;
+    __shared__ float s_inv[64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ns = a.nsplit;  // ns <= 64
+    float mi[16], li[16];  // rows w, w + 4, ...: split `lane`
+    constexpr int RW = 64 / kWaves;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) acc[i] = 0.0f;
+    for (int k = 0; k < RW; ++k) {
+        const int r = w + kWaves * k;
+        const float *ml = a.part_ml + ((row0 + min(r, n - 1)) * ns + min(lane, ns - 1)) * 2;
+        if (r < n) {
+            mi[k] = lane < ns ? ml[0] : -INFINITY;
+            li[k] = lane < ns ? ml[1] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < RW; ++k) {
+        const int r = w + kWaves * k;
+        if (r >= n) break;
+        float M = mi[k];
+        for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        // (a split without a key has max -inf and sum 0; one whose keys are NaN has a NaN sum)
+        const float wi = mi[k] == -INFINITY ? 0.0f : fast_exp2(mi[k] - M);
+        float L = li[k] != li[k] ? li[k] : wi * li[k];
+        for (int o = 32; o >= 1; o >>= 1) L += __shfl_xor(L, o, 64);
+        if (lane < ns) lds[r * ns + lane] = wi;
+        if (lane == 0) {
+            s_inv[r] = L == 0.0f ? 0.0f : 1.0f / L;
+            if (a.lse) a.lse[row0 + r] = L == 0.0f ? INFINITY : (M + log2f(L)) * kLn2;
+        }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < n * PIECES; e += 64 * kWaves) {
+        const int r = e / PIECES, d = 4 * (e % PIECES);
+        const float *po = a.part_o + (row0 + r) * ns * Dp + d;
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
         constexpr int U = 8;
         for (int s0 = 0; s0 < ns; s0 += U) {
-            float x[U][NI];
+            f32x4 x[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int i = 0; i < NI; ++i) x[u][i] = po[(int64_t)min(s0 + u, ns - 1) * Dp + 64 * i];
+            for (int u = 0; u < U; ++u) x[u] = *(const f32x4 *)(po + (int64_t)min(s0 + u, ns - 1) * Dp);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const float ws = s0 + u < ns ? __shfl(wi, min(s0 + u, ns - 1), 64) : 0.0f;
+                const float ws = s0 + u < ns ? lds[r * ns + s0 + u] : 0.0f;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) acc[i] = ws == 0.0f ? acc[i] : fmaf(ws, x[u][i], acc[i]);
+                for (int i = 0; i < 4; ++i) acc[i] = ws == 0.0f ? acc[i] : fmaf(ws, x[u][i], acc[i]);
             }
         }
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const float inv = s_inv[r];
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
-            if (lane + 64 * i < a.D) ((TO *)a.o)[row * a.D + lane + 64 * i] = (TO)(acc[i] * inv);
-        if (a.lse && lane == 0) a.lse[row] = L == 0.0f ? INFINITY : (M + log2f(L)) * kLn2;
+        for (int i = 0; i < 4; ++i)
+            if (d + i < a.D) ((TO *)a.o)[(row0 + r) * a.D + d + i] = (TO)(acc[i] * inv);
     }
+}
+
+// LDS of a launch: the wavefronts' rows on their way to being joined, or the splits' weights.
+GT_KVB_FN inline int64_t attn_lds_floats(int rows, int Dp, int nsplit) {
+    const int64_t join = 2 * (int64_t)rows * (Dp + 4), merge = (int64_t)rows * nsplit;
+    return join > merge ? join : merge;
 }
 
 template <typename QT, int NI, int CT, bool E4M3>
 __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
     constexpr bool F32 = __is_same(QT, float);
     constexpr int Dp = 64 * NI, COLS = 16 * CT, DT = 4 * NI;
-    constexpr int OP = Dp + 4;  // pitch of the joined rows
-    __shared__ float s_o[COLS * OP];
+    constexpr int OP = Dp + 4;  // pitch of the rows to be joined
+    extern __shared__ __attribute__((aligned(16))) float s_o[];  // [2][row]
     __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
     __shared__ int s_last;
 
@@ -240,23 +270,34 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     }
 
     // The softmax step over 64 keys from k0 on: c holds the column's products with the codes of keys 16 kb + 4g + i,
-    // ksc and vexp(kb, i) a key's scale and V exponent; every key at or above `end` is not there.  Leaves p' as
-    // operands and rescales the sums.
-    auto softmax = [&](f32x4(&c)[CT][4], int k0, int end, auto &&ksc, auto &&vexp, half8(&ph)[CT][2], half8(&pl)[CT][2]) {
-        const bool all = k0 + kUnit <= min(lim_all, end) && nr == COLS;
+    // ksc and vexp(kb, i) a key's scale and V exponent (PER_KEY: they differ within a kb); every key at or above
+    // `end` is not there.  Leaves p' as operands and rescales the sums.
+    auto softmax = [&](auto per_key, f32x4(&c)[CT][4], int k0, int end, auto &&ksc, auto &&vexp, half8(&ph)[CT][2], half8(&pl)[CT][2]) {
+        constexpr bool PER_KEY = decltype(per_key)::value;
+        const bool all = !PER_KEY && k0 + kUnit <= min(lim_all, end);
 #pragma unroll
         for (int ct = 0; ct < CT; ++ct) {
             float cm = -INFINITY, cv = -INFINITY;
+            if (all) {
+                // every row sees every key: the scales are positive, so a kb's largest s is its largest product's
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float s = c[ct][kb][i] * (f[ct] * ksc(kb, i));
-                    if (!all) s = k0 + 16 * kb + 4 * g + i < min(lim[ct], end) ? s : -INFINITY;
-                    c[ct][kb][i] = s;
+                for (int kb = 0; kb < 4; ++kb) {
+                    const f32x4 x = c[ct][kb];
+                    const float s = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * (f[ct] * ksc(kb, 0));
                     cm = fmaxf(cm, s);
-                    cv = fmaxf(cv, s + vexp(kb, i));
+                    cv = fmaxf(cv, s + vexp(kb, 0));
                 }
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float s = c[ct][kb][i] * (f[ct] * ksc(kb, i));
+                        c[ct][kb][i] = k0 + 16 * kb + 4 * g + i < min(lim[ct], end) ? s : -INFINITY;
+                        cm = fmaxf(cm, c[ct][kb][i]);
+                        cv = fmaxf(cv, c[ct][kb][i] + vexp(kb, i));
+                    }
+            }
             const float mn = fmaxf(m[ct], max_g(cm)), vn = fmaxf(mv[ct], max_g(cv));
             const float ms = mn == -INFINITY ? 0.0f : mn;
             const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m[ct] - mn);
@@ -266,19 +307,26 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
             mv[ct] = vn;
             float sum = 0.0f;
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
+            for (int kb = 0; kb < 4; ++kb) {
+                const float fk = f[ct] * ksc(kb, 0);
+                float up = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = fast_exp2(c[ct][kb][i] - ms);
+                    const float p = fast_exp2(all ? fmaf(c[ct][kb][i], fk, -ms) : c[ct][kb][i] - ms);
                     sum += p;
-                    // p <= 2^-100 next to a larger 2^c: nothing of the sum; a NaN exponent (a block that holds one) stays
-                    const float e = vexp(kb, i) - shift;
-                    const float pv = p == 0.0f ? 0.0f : p * fast_exp2(e > 100.0f ? 100.0f : e);
+                    // 2^(c - r): where it passes 2^100, p is 0 or next to it; a NaN (a block that holds one) stays
+                    if (i == 0 || PER_KEY) {
+                        const float e = vexp(kb, i) - shift;
+                        up = fast_exp2(e > 100.0f ? 100.0f : e);
+                    }
+                    float pv = p * up;
+                    if (!all) pv = p == 0.0f ? 0.0f : pv;  // (a key that is not seen adds nothing, NaN or not)
                     const int at = 4 * (kb & 1) + i;
                     const _Float16 hi = (_Float16)pv;
                     ph[ct][kb >> 1][at] = hi;
                     if constexpr (F32) pl[ct][kb >> 1][at] = (_Float16)(pv - (float)hi);
                 }
+            }
             lsum[ct] = fmaf(lsum[ct], alpha, sum_g(sum));
             if (__builtin_amdgcn_ballot_w64(beta != 1.0f) != 0) {
 #pragma unroll
@@ -289,22 +337,26 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
 
     // ---- whole blocks ----
     const int u0 = blockIdx.y * a.span, u1 = min(u0 + a.span, (full + kUnit - 1) / kUnit);
-    const int64_t slice = bg * a.units * kUnit * Dp;
-    const uint8_t *kc = a.k + slice + 16 * lane, *vc = a.v + slice + 16 * lane;
+    const int64_t from = (bg * a.units + u0) * kUnit * Dp;
+    // buffer loads: a uniform place, a lane's 16 bytes; past the last unit they return zeros and fetch nothing
+    const int bytes = max(u1 - u0, 0) * kUnit * Dp;  // (below 2^31: gt_kv_blocks_attn_supported)
+    const auto kr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + from), 0, bytes, 0x00027000);
+    const auto vr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + from), 0, bytes, 0x00027000);
     const int64_t nblk = a.units * kUnit / a.N;
     const float *sc = ((lane & 4) ? a.vs : a.ks) + bg * nblk;  // lanes 0..3 hold K's scales, 4..7 V's
     u32x4 rk[DT], rv[DT];
     float rs = 0.0f;
+    constexpr int kNonTemporal = 2;
     auto load_k = [&](int u) {
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            rk[t] = __builtin_nontemporal_load((const u32x4 *)(kc + (int64_t)u * kUnit * Dp + 1024 * t));
+            rk[t] = __builtin_amdgcn_raw_buffer_load_b128(kr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
         rs = sc[min((int64_t)(u * kUnit + 16 * (lane & 3)) / a.N, nblk - 1)];
     };
     auto load_v = [&](int u) {
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-            rv[t] = __builtin_nontemporal_load((const u32x4 *)(vc + (int64_t)u * kUnit * Dp + 1024 * t));
+            rv[t] = __builtin_amdgcn_raw_buffer_load_b128(vr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
     };
     f32x4 c[CT][4];
     float sk[4], ev[4];
@@ -312,8 +364,8 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
             sk[kb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rs), kb));
-            const uint32_t vb = __builtin_amdgcn_readlane(__float_as_uint(rs), 4 + kb);
-            ev[kb] = (vb >> 23) == 255 ? NAN : (float)((int)(vb >> 23) - 127);
+            ev[kb] = exponent_bits(__builtin_amdgcn_readlane(__float_as_uint(rs), 4 + kb));
+            __builtin_amdgcn_sched_barrier(0);  // (one tile's operands at a time: registers)
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -331,11 +383,12 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     };
     half8 ph[CT][2], pl[CT][2];
     auto weigh = [&](int u) {
-        softmax(c, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; }, ph, pl);
+        softmax(std::false_type{}, c, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; }, ph, pl);
     };
     auto values = [&]() {
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
+        for (int t = 0; t < DT; ++t) {
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const half8 va = decode8<E4M3>(rv[t][2 * j], rv[t][2 * j + 1]);
@@ -345,66 +398,47 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
                     acc[ct][t] = mma(va, ph[ct][j], acc[ct][t]);
                 }
             }
+        }
     };
     // the next unit's K is on its way during the softmax and P.V, its V during the next scores
-    int u = u0 + w;
-    if (u < u1) {
-        load_k(u);
-        load_v(u);
-        for (; u + kWaves < u1; u += kWaves) {
-            scores();
-            load_k(u + kWaves);
-            weigh(u);
-            values();
-            load_v(u + kWaves);
-        }
+    if (u0 + w < u1) {
+        load_k(u0 + w);
+        load_v(u0 + w);
+    }
+    for (int u = u0 + w; u < u1; u += kWaves) {
         scores();
+        load_k(u + kWaves);
         weigh(u);
         values();
+        load_v(u + kWaves);
     }
 
     // ---- the tail: by the last split that has units, as its next ones ----
     const int nu = max(u1 - u0, 0);
     const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && u1 * kUnit >= full;
+    const int room = max(a.N, kUnit);  // tokens of a plane of operands
     for (int tu = 0; mine && tu * kUnit < tail; ++tu) {
         if ((nu + tu) % kWaves != w) continue;
-        const float *kt = a.kt + bg * a.N * a.D, *vt = a.vt + bg * a.N * a.D;
         const int t0 = tu * kUnit;
-        float ksc[4][4], vex[4][4], vinv[4][4];
+        const _Float16 *kt = a.kt + (bg * 2 * room + t0) * Dp + 16 * lane, *vt = a.vt + (bg * 2 * room + t0) * Dp + 16 * lane;
+        const int64_t lo_at = (int64_t)room * Dp;
+        f32x4 ksc[4], vex[4];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-            // K row 16 kb + n of the unit; its scale goes to the lanes that hold its scores
-            const int t = t0 + 16 * kb + n;
-            float x[NI][16];
-            float amax = 0.0f;
-            bool odd = false;
+            ksc[kb] = *(const f32x4 *)(a.kts + bg * room + t0 + 16 * kb + 4 * g);
+            const f32x4 vs = *(const f32x4 *)(a.vts + bg * room + t0 + 16 * kb + 4 * g);
 #pragma unroll
-            for (int i = 0; i < NI; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int d = 16 * (4 * i + g) + e;
-                    x[i][e] = t < tail && d < a.D ? kt[(int64_t)t * a.D + d] : 0.0f;
-                    amax = fmaxf(amax, fabsf(x[i][e]));
-                    odd = odd || !(fabsf(x[i][e]) < INFINITY);
-                }
-            amax = max_g(odd ? INFINITY : amax);
-            odd = amax == INFINITY;
-            const int e2 = exponent_of(amax);
-            const float inv = pow2(-e2);
-            if (odd) {
-#pragma unroll
-                for (int i = 0; i < NI; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[i][e] = 0.0f;
-            }
+            for (int i = 0; i < 4; ++i) vex[kb][i] = exponent_bits(__float_as_uint(vs[i]));
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            __builtin_amdgcn_sched_barrier(0);  // (one tile's operands at a time: registers)
+            if (t0 + 16 * kb >= tail) continue;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    half8 hi, lo;
-                    split8(x[i] + 8 * j, inv, hi, lo);
+                    const half8 hi = *(const half8 *)(kt + kb * 16 * Dp + 1024 * i + 8 * j);
+                    const half8 lo = *(const half8 *)(kt + lo_at + kb * 16 * Dp + 1024 * i + 8 * j);
 #pragma unroll
                     for (int ct = 0; ct < CT; ++ct) {
                         if constexpr (F32) c[ct][kb] = mma(hi, ql[ct][i][j], c[ct][kb]);
@@ -412,43 +446,15 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
                         c[ct][kb] = mma(hi, qh[ct][i][j], c[ct][kb]);
                     }
                 }
-            const float ks = odd ? NAN : pow2(e2);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) ksc[kb][i] = __shfl(ks, 4 * g + i, 64);
-            // V rows 16 kb + 4g + i: the largest magnitude over the dims, of which this lane sees each 16th
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int tv = t0 + 16 * kb + 4 * g + i;
-                float vm = 0.0f;
-                bool vodd = false;
-                for (int d = n; d < a.D; d += 16) {
-                    const float y = tv < tail ? fabsf(vt[(int64_t)tv * a.D + d]) : 0.0f;
-                    vm = fmaxf(vm, y);
-                    vodd = vodd || !(y < INFINITY);
-                }
-                vm = vodd ? INFINITY : vm;
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) vm = fmaxf(vm, __shfl_xor(vm, o, 64));
-                const int ve = vm == 0.0f ? -126 : exponent_of(vm);
-                vex[kb][i] = vm == INFINITY ? NAN : (float)ve;
-                vinv[kb][i] = vm == INFINITY || vm == 0.0f ? 0.0f : pow2(-ve);
-            }
         }
-        softmax(c, full + t0, len, [&](int kb, int i) { return ksc[kb][i]; }, [&](int kb, int i) { return vex[kb][i]; }, ph, pl);
+        softmax(std::true_type{}, c, full + t0, len, [&](int kb, int i) { return ksc[kb][i]; }, [&](int kb, int i) { return vex[kb][i]; }, ph, pl);
 #pragma unroll
-        for (int t = 0; t < DT; ++t) {
-            const int d = 16 * t + n;
+        for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                half8 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int kb = 2 * j + (e >> 2), i = e & 3, tv = t0 + 16 * kb + 4 * g + i;
-                    const bool there = tv < tail && d < a.D && vinv[kb][i] != 0.0f;
-                    const float y = there ? vt[(int64_t)tv * a.D + d] * vinv[kb][i] : 0.0f;
-                    hi[e] = (_Float16)y;
-                    lo[e] = (_Float16)(y - (float)hi[e]);
-                }
+                if (j == 0) __builtin_amdgcn_sched_barrier(0);
+                if (t0 + 32 * j >= tail) continue;  // (operand j: tokens 32 j .. +31)
+                const half8 hi = *(const half8 *)(vt + 1024 * t + 8 * j), lo = *(const half8 *)(vt + lo_at + 1024 * t + 8 * j);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) {
                     if constexpr (F32) acc[ct][t] = mma(hi, pl[ct][j], acc[ct][t]);
@@ -456,7 +462,6 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
                     acc[ct][t] = mma(hi, ph[ct][j], acc[ct][t]);
                 }
             }
-        }
     }
 
     // ---- join the wavefronts, in order ----
@@ -467,22 +472,24 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
             s_l[w][16 * ct + n] = lsum[ct];
         }
     __syncthreads();
-    for (int ww = 0; ww < kWaves; ++ww) {
-        if (w == ww) {
+    // waves 2 and 3 leave theirs, waves 0 and 1 add their own
+#pragma unroll
+    for (int half = 1; half >= 0; --half) {
+        if ((w >> 1) == half) {
 #pragma unroll
             for (int ct = 0; ct < CT; ++ct) {
                 const int col = 16 * ct + n;
+                if (col >= nr) continue;
                 const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
                 const float to = mv[ct] == -INFINITY ? 0.0f : fast_exp2(mv[ct] - (M == -INFINITY ? 0.0f : M));
                 const bool bad = lsum[ct] != lsum[ct];
 #pragma unroll
-                for (int t = 0; t < DT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float *o = &s_o[col * OP + 16 * t + 4 * g + i];
-                        const float y = bad ? NAN : acc[ct][t][i] * to;
-                        *o = ww == 0 ? y : *o + y;
-                    }
+                for (int t = 0; t < DT; ++t) {
+                    f32x4 y = acc[ct][t] * to;
+                    if (bad) y = f32x4{NAN, NAN, NAN, NAN};
+                    f32x4 *o = (f32x4 *)&s_o[((w & 1) * nr + col) * OP + 16 * t + 4 * g];
+                    *o = half == 0 ? *o + y : y;
+                }
             }
         }
         __syncthreads();
@@ -491,13 +498,13 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     for (int e = threadIdx.x; e < nr * Dp; e += 64 * kWaves) {
         const int col = e / Dp, d = e - col * Dp;
         const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+        const float o = s_o[col * OP + d] + s_o[(nr + col) * OP + d];
         float L = 0.0f;
 #pragma unroll
         for (int ww = 0; ww < kWaves; ++ww) {
             const float lw = s_l[ww][col];
             L += s_m[ww][col] == -INFINITY ? (lw != lw ? lw : 0.0f) : fast_exp2(s_m[ww][col] - M) * lw;
         }
-        const float o = s_o[col * OP + d];
         const int64_t row = row0 + col;
         if (a.nsplit == 1) {
             if (d < a.D) ((QT *)a.o)[row * a.D + d] = (QT)(L == 0.0f ? 0.0f : o / L);
@@ -519,7 +526,7 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
         s_last = __hip_atomic_fetch_add(&a.counters[x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.nsplit - 1;
     __syncthreads();
     if (!s_last) return;
-    merge_splits<QT, NI>(a, row0, nr);
+    merge_splits<QT, NI>(a, row0, nr, s_o);
     if (threadIdx.x == 0) __hip_atomic_store(&a.counters[x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 

@@ -35,10 +35,10 @@ int64_t resident_groups(const void *kernel) {
 
 }  // namespace
 
-bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype) {
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int64_t max_len, int q_dtype) {
     const int64_t rows = H / c.Hkv * L;
     return (q_dtype == GT_F16 || q_dtype == GT_BF16 || q_dtype == GT_F32) && rows <= kKvBlocksAttnRows &&
-           c.B * H * L < (1LL << 31);
+           c.B * H * L < (1LL << 31) && (max_len + kUnit) * c.Dp < (1LL << 31);  // (32-bit offsets)
 }
 
 hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note) {
@@ -53,13 +53,15 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
     a.v = (const uint8_t *)c.codes[1];
     a.ks = c.scales[0];
     a.vs = c.scales[1];
-    a.kt = c.tail[0];
-    a.vt = c.tail[1];
+    a.kt = (const _Float16 *)c.ops[0];
+    a.vt = (const _Float16 *)c.ops[1];
+    a.kts = c.op_scales[0];
+    a.vts = c.op_scales[1];
     a.len = r.len;
     a.scale = r.scale;
     a.causal = r.causal;
     const int64_t per16 = r.q_dtype == GT_F32 ? 4 : 8;
-    a.q_vec = (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
+    a.q_vec = c.D % 16 == 0 && (uintptr_t)r.q % 16 == 0 && a.q_sb % per16 == 0 && a.q_sh % per16 == 0 && a.q_sl % per16 == 0;
     a.B = (int)c.B;
     a.H = (int)r.H;
     a.Hkv = (int)c.Hkv;
@@ -99,5 +101,6 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
            " rows=" + std::to_string(rows) + " columns=" + std::to_string(16 * ct) + " splits=" + std::to_string(n) +
            " units=" + std::to_string(grid);
     void *args[] = {(void *)&a};
-    return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3(64 * kWaves), args, 0, s);
+    const size_t lds = (size_t)attn_lds_floats((int)std::min<int64_t>(rows, 16 * ct), c.Dp, n) * sizeof(float);
+    return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3(64 * kWaves), args, lds, s);
 }

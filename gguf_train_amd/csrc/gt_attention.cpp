@@ -662,7 +662,7 @@ extern "C" gt_tensor *gt_flash_attention_rope(const gt_tensor *q, const gt_tenso
         gt_scratch table;
         gt_tensor *kr = pd ? tmp.keep(gt_new_tensor(4, kd->shape, kd->dtype, GT_DEV_CUDA, dev)) : nullptr;
         if (!kr || !gt_scratch_alloc(table, (size_t)need * (size_t)(D / 2) * 2 * sizeof(float), dev) ||
-            !gt_hip_check(gt_launch_rope_table((const int32_t *)gt_data(pd), nullptr, 1, need, n_dims,
+            !gt_hip_check(gt_launch_rope_table((const int32_t *)gt_data(pd), nullptr, nullptr, 1, need, n_dims,
                                                gt_rope_theta_scale(freq_base, n_dims), freq_scale, 0, table.ptr(),
                                                gt_stream()),
                           "rope table kernel") ||
@@ -1346,6 +1346,28 @@ extern "C" gt_tensor *gt_attention_weights_dropout(const gt_tensor *q, const gt_
 // 8-bit codes with a scale per block of tokens and head instead (kv_blocks.h).  Tokens can be evicted, by the
 // attention weight that they have accumulated; positions then run ahead of the lengths.
 
+// What a block cache holds, per K and V: the codes (B, Hkv, 64 units, Dp), the scales (B, Hkv, blocks), the tail
+// (B, Hkv, block, D) and, with R = max(block, 64), its operands (B, Hkv, 2, R, Dp) and their scales (B, Hkv, R).
+struct KvBlockMemory {
+    gt_tensor *codes[2] = {}, *scales[2] = {}, *tail[2] = {}, *ops[2] = {}, *op_scales[2] = {};
+    KvBlockMemory() = default;
+    KvBlockMemory(const KvBlockMemory &) = delete;
+    KvBlockMemory &operator=(const KvBlockMemory &) = delete;
+    ~KvBlockMemory() {
+        for (int i = 0; i < 2; ++i)
+            for (gt_tensor *t : {codes[i], scales[i], tail[i], ops[i], op_scales[i]}) gt_tensor_free(t);
+    }
+    void swap(KvBlockMemory &o) {
+        for (int i = 0; i < 2; ++i) {
+            std::swap(codes[i], o.codes[i]);
+            std::swap(scales[i], o.scales[i]);
+            std::swap(tail[i], o.tail[i]);
+            std::swap(ops[i], o.ops[i]);
+            std::swap(op_scales[i], o.op_scales[i]);
+        }
+    }
+};
+
 struct gt_kv_cache {
     int64_t B = 0, Hkv = 0, cap = 0, D = 0;
     int dtype = GT_F16;
@@ -1355,16 +1377,15 @@ struct gt_kv_cache {
     // device copy of len (int32, B), and the array that the next append writes the new lengths to (its
     // workgroups still read the old ones); the two swap, so nothing is uploaded
     gt_tensor *len_dev = nullptr, *len_next = nullptr;
-    // a block cache (dtype GT_I8 or GT_F8E4M3; k and v null): tokens per block, and per K and V the codes (B, Hkv,
-    // 64 units, Dp), the scales (B, Hkv, blocks) and the tail (B, Hkv, block, D)
+    // a block cache (dtype GT_I8 or GT_F8E4M3; k and v null): tokens per block, and its memory
     int block = 0, Dp = 0;
     int64_t units = 0;
-    gt_tensor *codes[2] = {}, *scales[2] = {}, *tail[2] = {};
+    KvBlockMemory mem;
     int src_dtype = -1;  // the dtype of every row appended since the cache was empty (GT_F32: several)
-    // the position after each sequence's last token: len and the evicted tokens; on the device (as len) once
-    // there are any
+    // the position after each sequence's last token: its length and the tokens evicted, whose number is on the
+    // device too once there are any
     std::vector<int32_t> seen;
-    gt_tensor *seen_dev = nullptr, *seen_next = nullptr;
+    gt_tensor *evicted = nullptr;
     gt_tensor *sums = nullptr;  // accumulated attention weights (B, Hkv, cap) float32, zeros past the lengths
 };
 
@@ -1386,6 +1407,22 @@ R guarded(R failed, F &&body) {
 bool kv_zero(gt_tensor *t) {
     return gt_hip_check(gt_launch_fill_zero(gt_data(t), (int64_t)gt_dtype_nbytes(t->dtype, t->numel), gt_stream()),
                         "kv cache: zero fill");
+}
+
+// Memory of a block cache's sizes, for a cache without tokens (empty) or about to be given its tokens.
+bool kv_block_memory(const gt_kv_cache *c, KvBlockMemory &m, bool empty) {
+    const int64_t room = std::max(c->block, gtkvb::kUnit), tokens = c->units * gtkvb::kUnit;
+    const int64_t codes[4] = {c->B, c->Hkv, tokens, c->Dp}, scales[3] = {c->B, c->Hkv, tokens / c->block};
+    const int64_t tail[4] = {c->B, c->Hkv, c->block, c->D}, ops[5] = {c->B, c->Hkv, 2, room, c->Dp}, op_scales[3] = {c->B, c->Hkv, room};
+    auto make = [&](int n, const int64_t *shape, int dtype) { return gt_new_tensor(n, shape, dtype, GT_DEV_CUDA, c->dev); };
+    for (int i = 0; i < 2; ++i) {
+        if (!(m.codes[i] = make(4, codes, GT_U8)) || !(m.scales[i] = make(3, scales, GT_F32)) || !(m.tail[i] = make(4, tail, GT_F32)) ||
+            !(m.ops[i] = make(5, ops, GT_F16)) || !(m.op_scales[i] = make(3, op_scales, GT_F32)))
+            return false;
+        // operands of tokens past the tail meet weights of 0: they have to be finite
+        if (empty && !kv_zero(m.ops[i])) return false;
+    }
+    return true;
 }
 
 bool kv_check_rows(const char *who, const gt_kv_cache *c, const gt_tensor *t, const char *name) {
@@ -1502,15 +1539,8 @@ extern "C" gt_kv_cache *gt_kv_cache_create_blocks(int64_t batch, int64_t n_head_
         c->units = tokens / gtkvb::kUnit;
         c->len.assign((size_t)batch, 0);
         c->seen.assign((size_t)batch, 0);
-        const int64_t csh[4] = {batch, n_head_kv, tokens, c->Dp}, ssh[3] = {batch, n_head_kv, tokens / block_tokens};
-        const int64_t tsh[4] = {batch, n_head_kv, block_tokens, head_dim}, lsh[1] = {batch};
-        for (int i = 0; i < 2; ++i) {
-            if (!(c->codes[i] = gt_new_tensor(4, csh, GT_U8, GT_DEV_CUDA, device_index)) ||
-                !(c->scales[i] = gt_new_tensor(3, ssh, GT_F32, GT_DEV_CUDA, device_index)) ||
-                !(c->tail[i] = gt_new_tensor(4, tsh, GT_F32, GT_DEV_CUDA, device_index)) || !kv_zero(c->codes[i]) ||
-                !kv_zero(c->scales[i]) || !kv_zero(c->tail[i]))
-                return nullptr;  // (codes of tokens not yet written meet weights of 0: no NaN among them)
-        }
+        const int64_t lsh[1] = {batch};
+        if (!kv_block_memory(c.get(), c->mem, true)) return nullptr;
         if (!(c->len_dev = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, device_index)) ||
             !(c->len_next = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, device_index)) || !kv_zero(c->len_dev))
             return nullptr;
@@ -1520,9 +1550,7 @@ extern "C" gt_kv_cache *gt_kv_cache_create_blocks(int64_t batch, int64_t n_head_
 
 extern "C" void gt_kv_cache_free(gt_kv_cache *c) {
     if (!c) return;
-    for (gt_tensor *t : {c->k, c->v, c->len_dev, c->len_next, c->codes[0], c->codes[1], c->scales[0], c->scales[1], c->tail[0],
-                         c->tail[1], c->seen_dev, c->seen_next, c->sums})
-        gt_tensor_free(t);
+    for (gt_tensor *t : {c->k, c->v, c->len_dev, c->len_next, c->evicted, c->sums}) gt_tensor_free(t);
     delete c;
 }
 
@@ -1548,7 +1576,7 @@ extern "C" int gt_kv_cache_clear(gt_kv_cache *c, int64_t seq) {
         return gt_hip_check(gt_launch_fill_zero((char *)base + from * bytes, n * bytes, gt_stream()), "kv cache clear kernel");
     };
     if (!zero(len, sizeof(int32_t))) return -1;
-    if (c->seen_dev && !zero(gt_data(c->seen_dev), sizeof(int32_t))) return -1;
+    if (c->evicted && !zero(gt_data(c->evicted), sizeof(int32_t))) return -1;
     if (c->sums && !zero(gt_data(c->sums), c->Hkv * c->cap * (int64_t)sizeof(float))) return -1;
     return 0;
 }
@@ -1604,12 +1632,14 @@ struct KvRope {
     float freq_base, freq_scale;
 };
 
-gt_kv_blocks kv_blocks_of(const gt_kv_cache *c) {
+gt_kv_blocks kv_blocks_of(const gt_kv_cache *c, const KvBlockMemory &m) {
     gt_kv_blocks r{};
     for (int i = 0; i < 2; ++i) {
-        r.codes[i] = gt_data(c->codes[i]);
-        r.scales[i] = (float *)gt_data(c->scales[i]);
-        r.tail[i] = (float *)gt_data(c->tail[i]);
+        r.codes[i] = gt_data(m.codes[i]);
+        r.scales[i] = (float *)gt_data(m.scales[i]);
+        r.tail[i] = (float *)gt_data(m.tail[i]);
+        r.ops[i] = gt_data(m.ops[i]);
+        r.op_scales[i] = (float *)gt_data(m.op_scales[i]);
     }
     r.B = c->B;
     r.Hkv = c->Hkv;
@@ -1626,13 +1656,6 @@ int kv_advance(gt_kv_cache *c, int64_t T) {
     std::swap(c->len_dev, c->len_next);
     for (auto &n : c->len) n += (int32_t)T;
     for (auto &n : c->seen) n += (int32_t)T;
-    if (c->seen_dev) {
-        if (!gt_hip_check(gt_launch_kv_advance((const int32_t *)gt_data(c->seen_dev), (int32_t *)gt_data(c->seen_next), T, c->B,
-                                               gt_stream()),
-                          "kv cache positions kernel"))
-            return -1;
-        std::swap(c->seen_dev, c->seen_next);
-    }
     return 0;
 }
 
@@ -1649,11 +1672,11 @@ int kv_blocks_append(gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int
     gt_scratch table;
     if (rope) {
         const float theta_scale = gt_rope_theta_scale(rope->freq_base, rope->n_dims);
-        const int32_t *base = c->seen_dev ? (const int32_t *)gt_data(c->seen_dev) : pos;
+        const int32_t *evicted = c->evicted ? (const int32_t *)gt_data(c->evicted) : nullptr;
         const int64_t sh[4] = {c->B, c->Hkv, T, c->D};
         gt_tensor *turned = tmp.keep(gt_new_tensor(4, sh, src[0]->dtype, GT_DEV_CUDA, c->dev));
         if (!turned || !gt_scratch_alloc(table, (size_t)(c->B * T) * (size_t)rope->n_dims * sizeof(float), c->dev) ||
-            !gt_hip_check(gt_launch_rope_table(nullptr, base, T, c->B * T, rope->n_dims, theta_scale, rope->freq_scale, 0, table.ptr(),
+            !gt_hip_check(gt_launch_rope_table(nullptr, pos, evicted, T, c->B * T, rope->n_dims, theta_scale, rope->freq_scale, 0, table.ptr(),
                                                gt_stream()),
                           "rope table kernel") ||
             !gt_hip_check(gt_launch_rope(gt_data(src[0]), src[0]->dtype, src[0]->strides, gt_data(turned), table.ptr(), T, c->B, c->Hkv,
@@ -1665,12 +1688,13 @@ int kv_blocks_append(gt_kv_cache *c, const gt_tensor *k, const gt_tensor *v, int
     const bool one = src[0]->dtype == src[1]->dtype && src[0]->dtype != GT_F64;
     for (const gt_tensor *&t : src)
         if (!one && t->dtype != GT_F32 && !(t = tmp.keep(gt_to_device_dense(t, c->dev, GT_F32)))) return -1;
-    int64_t blocks = 0;
-    for (int32_t n : c->len) blocks = std::max<int64_t>(blocks, (n + T) / c->block - n / c->block);
+    const int64_t nt = std::max(c->block, gtkvb::kUnit);
+    int64_t groups = 1;
+    for (int32_t n : c->len) groups = std::max<int64_t>(groups, (n + T - 1) / nt - n / nt + 1);
     const void *data[2] = {gt_data(src[0]), gt_data(src[1])};
     const int64_t *strides[2] = {src[0]->strides, src[1]->strides};
-    if (!gt_hip_check(gt_launch_kv_blocks_append(kv_blocks_of(c), data, src[0]->dtype, strides, pos, nullptr,
-                                                 (int32_t *)gt_data(c->len_next), T, blocks, gt_stream()),
+    if (!gt_hip_check(gt_launch_kv_blocks_append(kv_blocks_of(c, c->mem), data, src[0]->dtype, strides, pos,
+                                                 (int32_t *)gt_data(c->len_next), T, groups, gt_stream()),
                       "kv cache block append kernel"))
         return -1;
     c->src_dtype = c->src_dtype < 0 || c->src_dtype == src[0]->dtype ? src[0]->dtype : GT_F32;
@@ -1720,7 +1744,7 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
     Temps tmp;
     const int32_t *pos = (const int32_t *)gt_data(c->len_dev);
     int32_t *next = (int32_t *)gt_data(c->len_next);
-    const int32_t *angle_pos = c->seen_dev ? (const int32_t *)gt_data(c->seen_dev) : pos;
+    const int32_t *evicted = c->evicted ? (const int32_t *)gt_data(c->evicted) : nullptr;
     gt_scratch table;
     // keys and values of one half or float32 dtype in aligned rows: one launch, which also forms the
     // angles of a few rows and the lengths after it
@@ -1731,10 +1755,10 @@ int kv_append(const char *who, gt_kv_cache *c, const gt_tensor *k, const gt_tens
                       gt_kv_append_vec_ok(gt_data(k), k->dtype, k->strides, gt_data(c->k), c->dtype, c->Hkv, T, c->D, n_dims) &&
                       gt_kv_append_vec_ok(gt_data(v), v->dtype, v->strides, gt_data(c->v), c->dtype, c->Hkv, T, c->D, 0);
     gt_rope_apply ra{};
-    if (rope && !(pair && !c->seen_dev && gt_kv_rope_inline(c->B, c->Hkv, T, c->D))) {
+    if (rope && !(pair && !evicted && gt_kv_rope_inline(c->B, c->Hkv, T, c->D))) {
         // (cos, sin) of table row b * T + t at the position of sequence b's next token + t
         if (!gt_scratch_alloc(table, (size_t)(c->B * T) * (size_t)(rope->n_dims / 2) * 2 * sizeof(float), c->dev) ||
-            !gt_hip_check(gt_launch_rope_table(nullptr, angle_pos, T, c->B * T, rope->n_dims,
+            !gt_hip_check(gt_launch_rope_table(nullptr, pos, evicted, T, c->B * T, rope->n_dims,
                                                gt_rope_theta_scale(rope->freq_base, rope->n_dims), rope->freq_scale, 0,
                                                table.ptr(), gt_stream()),
                           "rope table kernel"))
@@ -1828,8 +1852,8 @@ gt_tensor *kv_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_
     bool ok = true;
     int q8 = 0;
     if (c->block && o->numel > 0) {
-        const gt_kv_blocks blocks = kv_blocks_of(c);
-        if (gt_kv_blocks_attn_supported(blocks, H, L, q->dtype)) {
+        const gt_kv_blocks blocks = kv_blocks_of(c, c->mem);
+        if (gt_kv_blocks_attn_supported(blocks, H, L, maxlen, q->dtype)) {
             const gt_tensor *qs = stage(q, dev, q->dtype, tmp);
             ok = qs != nullptr;
             if (ok) {
@@ -1869,7 +1893,7 @@ gt_tensor *kv_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_
             gt_tensor *rk = tmp.keep(gt_new_tensor(4, vsh, kd, GT_DEV_CUDA, dev));
             gt_tensor *rv = tmp.keep(gt_new_tensor(4, vsh, kd, GT_DEV_CUDA, dev));
             ok = rk && rv &&
-                 gt_hip_check(gt_launch_kv_blocks_read(kv_blocks_of(c), kv_len, nullptr, maxlen, gt_data(rk), gt_data(rv), kd, gt_stream()),
+                 gt_hip_check(gt_launch_kv_blocks_read(kv_blocks_of(c, c->mem), kv_len, maxlen, gt_data(rk), gt_data(rv), kd, gt_stream()),
                               "kv cache block read kernel");
             kv_views[0] = rk;
             kv_views[1] = rv;
@@ -1982,7 +2006,7 @@ gt_tensor *kv_attention_accumulate(gt_kv_cache *c, const gt_tensor *q, float sca
     gt_tensor *o = kv_attention(c, q, scale, is_causal, lse);
     if (!o) return nullptr;
     const gt_tensor *qs = stage(q, c->dev, q->dtype, tmp);
-    const gt_kv_blocks blocks = c->block ? kv_blocks_of(c) : gt_kv_blocks{};
+    const gt_kv_blocks blocks = c->block ? kv_blocks_of(c, c->mem) : gt_kv_blocks{};
     gt_key_weights r{};
     if (qs) {
         r.q = gt_data(qs);
@@ -2054,64 +2078,47 @@ int kv_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weig
     const int64_t ksh[3] = {B, Hkv, keep}, lsh[1] = {B};
     gt_tensor *kept = gt_new_tensor(3, ksh, GT_I64, GT_DEV_CUDA, c->dev);
     if (!kept) return -1;
-    gt_tensor *owned = kept_out ? nullptr : tmp.keep(kept);
-    (void)owned;
+    if (!kept_out) tmp.keep(kept);
     const int32_t *len = (const int32_t *)gt_data(c->len_dev);
     const int64_t *places = (const int64_t *)gt_data(kept);
-    bool ok = gt_hip_check(gt_launch_kv_select((const float *)gt_data(w), w->strides, len, (int64_t *)gt_data(kept), B, Hkv, keep, recent,
-                                               gt_stream()),
-                           "kv cache select kernel");
-    if (ok && max_len > keep) {
-        gt_tensor *count = tmp.keep(gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev));
-        // positions, which lengths no longer tell
-        if (!c->seen_dev) {
-            gt_tensor *a = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev), *b = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev);
-            ok = a && b && gt_hip_check(gt_launch_kv_advance(len, (int32_t *)gt_data(a), 0, B, gt_stream()), "kv cache positions kernel");
-            if (ok) {
-                c->seen_dev = a;
-                c->seen_next = b;
-            } else {
-                gt_tensor_free(a);
-                gt_tensor_free(b);
-            }
-        }
-        ok = ok && count &&
-             gt_hip_check(gt_launch_kv_evict_lengths(len, (int32_t *)gt_data(c->len_next), (int32_t *)gt_data(count), keep, B, gt_stream()),
-                          "kv cache lengths kernel");
-        gt_kv_moved moved[3];
-        int n = 0, zeroed = -1;
-        auto move = [&](gt_tensor *rows, int64_t row_bytes) {
-            const int64_t sh[1] = {B * Hkv * keep * row_bytes};
-            gt_tensor *t = tmp.keep(gt_new_tensor(1, sh, GT_U8, GT_DEV_CUDA, c->dev));
-            if (t) moved[n++] = {gt_data(rows), gt_data(t), row_bytes};
-            return t != nullptr;
-        };
-        if (ok && c->block) {
-            // the kept tokens' values, quantized again in their new blocks (exactly, where the scale stays)
-            const gt_kv_blocks blocks = kv_blocks_of(c);
-            const int64_t sh[4] = {B, Hkv, keep, c->D};
-            gt_tensor *kv[2];
-            for (gt_tensor *&t : kv) ok = ok && (t = tmp.keep(gt_new_tensor(4, sh, GT_F32, GT_DEV_CUDA, c->dev)));
-            ok = ok && gt_hip_check(gt_launch_kv_blocks_read(blocks, len, places, keep, gt_data(kv[0]), gt_data(kv[1]), GT_F32, gt_stream()),
-                                    "kv cache block read kernel");
-            if (ok) {
-                const void *data[2] = {gt_data(kv[0]), gt_data(kv[1])};
-                const int64_t *strides[2] = {kv[0]->strides, kv[1]->strides};
-                ok = gt_hip_check(gt_launch_kv_blocks_append(blocks, data, GT_F32, strides, nullptr, (const int32_t *)gt_data(count),
-                                                             nullptr, 0, keep / c->block, gt_stream()),
-                                  "kv cache block append kernel");
-            }
-        } else if (ok) {
-            const int64_t rb = (int64_t)gt_dtype_nbytes(c->dtype, c->D);
-            ok = move(c->k, rb) && move(c->v, rb);
-        }
+    // all memory first, so that what fails leaves the cache as it was
+    const bool cut = max_len > keep;
+    bool ok = true;
+    KvBlockMemory next;
+    gt_kv_moved moved[3];
+    int n = 0, zeroed = -1;
+    auto move = [&](gt_tensor *rows, int64_t row_bytes) {
+        const int64_t sh[1] = {B * Hkv * keep * row_bytes};
+        gt_tensor *t = tmp.keep(gt_new_tensor(1, sh, GT_U8, GT_DEV_CUDA, c->dev));
+        if (t) moved[n++] = {gt_data(rows), gt_data(t), row_bytes};
+        return t != nullptr;
+    };
+    if (cut) {
+        const int64_t rb = c->block ? 0 : (int64_t)gt_dtype_nbytes(c->dtype, c->D);
+        ok = c->block ? kv_block_memory(c, next, false) : move(c->k, rb) && move(c->v, rb);
         if (ok && c->sums) {
             zeroed = n;
             ok = move(c->sums, sizeof(float));
         }
-        ok = ok && gt_hip_check(gt_launch_kv_move(moved, n, zeroed, places, len, B, Hkv, keep, max_len, c->cap, gt_stream()),
-                                "kv cache move kernel");
+        if (ok && !c->evicted) {
+            c->evicted = gt_new_tensor(1, lsh, GT_I32, GT_DEV_CUDA, c->dev);
+            ok = c->evicted && kv_zero(c->evicted);
+        }
+    }
+    ok = ok && gt_hip_check(gt_launch_kv_select((const float *)gt_data(w), w->strides, len, (int32_t *)gt_data(c->len_next),
+                                                c->evicted ? (int32_t *)gt_data(c->evicted) : nullptr, (int64_t *)gt_data(kept), B, Hkv,
+                                                keep, recent, gt_stream()),
+                            "kv cache select kernel");
+    if (cut) {
+        // a block cache's kept tokens are quantized again in their new blocks (exactly where the scale stays or
+        // falls), in memory that takes the old one's place
+        ok = ok &&
+             (!c->block ||
+              gt_hip_check(gt_launch_kv_blocks_evict(kv_blocks_of(c, c->mem), kv_blocks_of(c, next), len, places, keep, gt_stream()),
+                           "kv cache block evict kernel")) &&
+             gt_hip_check(gt_launch_kv_move(moved, n, zeroed, places, len, B, Hkv, keep, max_len, c->cap, gt_stream()), "kv cache move kernel");
         if (ok) {
+            if (c->block) c->mem.swap(next);
             std::swap(c->len_dev, c->len_next);
             for (auto &x : c->len) x = (int32_t)std::min<int64_t>(x, keep);
         }
@@ -2141,7 +2148,7 @@ int kv_read(gt_kv_cache *c, int dtype, gt_tensor **k, gt_tensor **v) {
     const int32_t *len = (const int32_t *)gt_data(c->len_dev);
     bool ok = a && b;
     if (ok && rows > 0)
-        ok = gt_hip_check(c->block ? gt_launch_kv_blocks_read(kv_blocks_of(c), len, nullptr, rows, gt_data(a), gt_data(b), dtype, gt_stream())
+        ok = gt_hip_check(c->block ? gt_launch_kv_blocks_read(kv_blocks_of(c, c->mem), len, rows, gt_data(a), gt_data(b), dtype, gt_stream())
                                    : gt_launch_kv_rows_read(gt_data(c->k), gt_data(c->v), c->dtype, len, gt_data(a), gt_data(b), dtype,
                                                             c->B, c->Hkv, rows, c->D, c->cap, gt_stream()),
                           "kv cache read kernel");

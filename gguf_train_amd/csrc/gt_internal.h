@@ -151,8 +151,9 @@ hipError_t gt_launch_kv_advance(const int32_t *pos, int32_t *pos_next, int64_t T
 hipError_t gt_launch_kv_append_blocks(const void *src, void *dst, const int32_t *pos, int64_t B, int64_t Hkv,
                                       int64_t T, int64_t D, int64_t cap, hipStream_t stream);
 // RoPE angle table: (cos, sin) of pair i < n_dims/2 for `rows` positions, row r at position pos[r],
-// or base[r / T] + r % T when base is non-null; float2 per entry, sin negated when backward.
-hipError_t gt_launch_rope_table(const int32_t *pos, const int32_t *base, int64_t T, int64_t rows, int n_dims,
+// or base[r / T] (+ more[r / T] when given) + r % T when base is non-null; float2 per entry, sin negated when
+// backward.
+hipError_t gt_launch_rope_table(const int32_t *pos, const int32_t *base, const int32_t *more, int64_t T, int64_t rows, int n_dims,
                                 float theta_scale, float freq_scale, int backward, void *table, hipStream_t stream);
 // RoPE rotation of x (B, H, S, D; element strides) into the dense y of the same float dtype, with
 // the angles of table row b * table_b_stride + s; mode 0 NORMAL, 2 NEOX.
@@ -171,20 +172,26 @@ hipError_t gt_launch_rope(const void *x, int dtype, const int64_t *strides, void
 struct gt_kv_blocks {
     void *codes[2];
     float *scales[2], *tail[2];
+    void *ops[2];  // the tail's operands (float16)
+    float *op_scales[2];
     int64_t B, Hkv, D, units;
     int N, Dp;
     bool e4m3;
 };
-// Appends count[b] (null: T) rows of src[0] and src[1] (B, Hkv, T, D; float32, float16 or bfloat16, element
-// strides) after the pos[b] (null: 0) tokens that each sequence holds, quantizing the blocks that become
-// full, at most `blocks` of a sequence; pos_next[b] (null: not) becomes the tokens held afterwards.
+// Appends T rows of src[0] and src[1] (B, Hkv, T, D; float32, float16 or bfloat16, element strides) after the
+// pos[b] tokens that each sequence holds, quantizing the blocks that become full; pos_next[b] becomes the tokens
+// held afterwards.  `groups`: of max(N, 64) tokens that a sequence's new ones and the block in progress touch.
 hipError_t gt_launch_kv_blocks_append(const gt_kv_blocks &c, const void *const *src, int src_dtype,
-                                      const int64_t *const *strides, const int32_t *pos, const int32_t *count,
-                                      int32_t *pos_next, int64_t T, int64_t blocks, hipStream_t s);
-// The values of tokens 0 .. rows - 1, or kept[b, g, 0 .. rows - 1], as dense (B, Hkv, rows, D) float32, float16
-// or bfloat16; zeros for tokens that are not held.
-hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, const int64_t *kept, int64_t rows,
-                                    void *k, void *v, int dtype, hipStream_t s);
+                                      const int64_t *const *strides, const int32_t *pos, int32_t *pos_next, int64_t T,
+                                      int64_t groups, hipStream_t s);
+// The tokens kept[b, g, 0 .. min(len[b], keep) - 1] of `from`, in that order, as all that `to` (another cache's
+// memory of the same sizes) holds.
+hipError_t gt_launch_kv_blocks_evict(const gt_kv_blocks &from, const gt_kv_blocks &to, const int32_t *len, const int64_t *kept,
+                                     int64_t keep, hipStream_t s);
+// The values of tokens 0 .. rows - 1 as dense (B, Hkv, rows, D) float32, float16 or bfloat16; zeros for tokens
+// that are not held.
+hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, int64_t rows, void *k, void *v, int dtype,
+                                    hipStream_t s);
 // Attention of few rows over the block cache (attn_kv_blocks.h): q (B, H, L, D) with contiguous dims, o dense of
 // q's dtype, lse (B, H, L) or null.  `note` describes the launch.
 constexpr int64_t kKvBlocksAttnRows = 128;
@@ -197,7 +204,7 @@ struct gt_kv_blocks_attn {
     int q_dtype, causal;
     float scale;
 };
-bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype);
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int64_t max_len, int q_dtype);
 hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note);
 // Sums of the attention weights of a cache's tokens (attn_key_weights.hip): sums (B, Hkv, cap) becomes keep *
 // sums + the weights' sums over the rows of q and the heads of a group, from the attention's lse.  The keys:
@@ -216,9 +223,9 @@ struct gt_key_weights {
 hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s);
 // Eviction (kv_rows.hip).  Select: kept (B, Hkv, keep) = the tokens that stay, the `recent` last and those of the
 // largest weights w (element strides), in order; a sequence of at most `keep` tokens keeps them (-1 behind).
-hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int64_t *kept, int64_t B, int64_t Hkv,
-                               int64_t keep, int64_t recent, hipStream_t s);
-hipError_t gt_launch_kv_evict_lengths(const int32_t *len, int32_t *next, int32_t *count, int64_t keep, int64_t B, hipStream_t s);
+// next[b]: the length afterwards; evicted[b] grows by what is lost (null: no sequence is longer than keep).
+hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int32_t *next, int32_t *evicted, int64_t *kept,
+                               int64_t B, int64_t Hkv, int64_t keep, int64_t recent, hipStream_t s);
 // Moves the kept rows of up to 3 tensors (B, Hkv, cap) together, through scratch (B, Hkv, keep); zeroed: the
 // one (4-byte rows) whose places left behind become zero, or -1.
 struct gt_kv_moved {

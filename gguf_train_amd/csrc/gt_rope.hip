@@ -46,15 +46,15 @@ __device__ inline T from_f(float v) {
 }
 
 // (cos, sin) of every (table row, pair): row r is position pos[r], or base[r / T] + r % T when
-// base is given (rows appended after what each sequence holds).
-__global__ void rope_table_kernel(const int32_t *__restrict__ pos, const int32_t *__restrict__ base, int64_t T,
+// base is given (rows appended after what each sequence holds), `more` behind it (what it has lost) if given.
+__global__ void rope_table_kernel(const int32_t *__restrict__ pos, const int32_t *__restrict__ base, const int32_t *__restrict__ more, int64_t T,
                                   int64_t rows, int half, float theta_scale, float freq_scale, float sin_sign,
                                   float2 *__restrict__ table) {
     const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (idx >= rows * half) return;
     const int64_t r = idx / half;
     const int i = (int)(idx - r * half);
-    const int32_t p = base ? base[r / T] + (int32_t)(r % T) : pos[r];
+    const int32_t p = base ? base[r / T] + (more ? more[r / T] : 0) + (int32_t)(r % T) : pos[r];
     const float2 cs = rope_cos_sin(rope_theta(p, i, theta_scale), freq_scale);
     table[idx] = make_float2(cs.x, sin_sign * cs.y);
 }
@@ -184,14 +184,14 @@ hipError_t dispatch_rotation(const RopeArgs &a, int64_t numel, hipStream_t strea
 
 }  // namespace
 
-hipError_t gt_launch_rope_table(const int32_t *pos, const int32_t *base, int64_t T, int64_t rows, int n_dims,
+hipError_t gt_launch_rope_table(const int32_t *pos, const int32_t *base, const int32_t *more, int64_t T, int64_t rows, int n_dims,
                                 float theta_scale, float freq_scale, int backward, void *table, hipStream_t stream) {
     const int half = n_dims / 2;
     const int64_t n = rows * half;
     if (n <= 0) return hipSuccess;
     const int64_t blocks = (n + 255) / 256;
     if (blocks > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, pos, base, T, rows, half,
+    hipLaunchKernelGGL(rope_table_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, pos, base, more, T, rows, half,
                        theta_scale, freq_scale, backward ? -1.0f : 1.0f, (float2 *)table);
     return hipGetLastError();
 }

@@ -121,7 +121,7 @@ gt_tensor *rope_run(const gt_tensor *x, const gt_tensor *pos, const RopeLayout &
                           "rope kernel");
     } else if (ok) {
         ok = gt_scratch_alloc(table, (size_t)L.S * (size_t)(n_dims / 2) * 2 * sizeof(float), dev) &&
-             gt_hip_check(gt_launch_rope_table((const int32_t *)gt_data(ps), nullptr, 1, L.S, n_dims, theta_scale,
+             gt_hip_check(gt_launch_rope_table((const int32_t *)gt_data(ps), nullptr, nullptr, 1, L.S, n_dims, theta_scale,
                                                freq_scale, backward ? 1 : 0, table.ptr(), gt_stream()),
                           "rope table kernel") &&
              gt_hip_check(gt_launch_rope(gt_data(xs), x->dtype, strides, gt_data(out), table.ptr(), 0, L.B, L.H, L.S,

@@ -15,6 +15,7 @@
 //   V: units of 64 tokens; the 16 bytes at 16 l of KiB i are dim 16 i + m of tokens 16 kb + 4g + r at byte 4 kb + r
 //      (kb, r < 4), the A operands (dims x keys) of two, whose keys are those of which lane l holds the
 //      probabilities when the score product ends.
+// int8 codes are kept as code + 128 (the bytes that place themselves under a float16 exponent).
 // Dims are padded with zeros to Dp, a multiple of 64 (one of 64, 128 or 256).  Plain arithmetic that a host
 // program can check.
 #pragma once

@@ -1,14 +1,16 @@
-// The 8-bit block cache (kv_blocks.h): appending tokens (quantizing the blocks that become full) and reading
-// back the values that it stands for.
+// The 8-bit block cache (kv_blocks.h): appending tokens (quantizing the blocks that become full), moving the
+// tokens that an eviction leaves together, and reading back the values that the cache stands for.
 //
-// Append, bound by HBM (the rows once, a byte per value back): a workgroup owns a block of one sequence and
-// head.  It reads the block's rows twice, for the largest magnitude and to quantize, the second time from the
-// caches (a block of 32 tokens and 128 dims is 8 KiB of float16).
+// Append, bound by HBM (the rows once, a byte per value back): a workgroup owns 64 tokens of one sequence and
+// head (128 where a block has as many) and keeps their values in registers between the largest magnitude and
+// the codes, so a row is read once.  A thread's 16 values are 16 dims of a token for K and 4 tokens x 4 dims for
+// V, what lies together in the codes' order.  An eviction is the same with the old cache's tokens for source.
 // Read, bound by HBM (mostly the values written): a workgroup stages a unit of 64 tokens' codes in LDS, from
 // which each thread gathers 8 dims of a token.
 
 #include "gt_internal.h"
 #include "kv_blocks.h"
+#include "vec_dims.h"
 
 #include <algorithm>
 
@@ -29,28 +31,22 @@ __device__ inline T from_f(float x) {
     return (T)x;
 }
 
-// 16 dims of a row from d0 on as float32, zeros from D on; VEC: contiguous, 16-byte aligned, D % 16 == 0.
+// 16 dims of a row from d0 on as float32, zeros from D on; VEC: contiguous, 16-byte aligned, D % 16 == 0.  (No
+// branch around a load: several are in flight.)
 template <typename T, bool VEC>
-__device__ inline void load16(const T *row, int64_t sd, int d0, int D, float *v) {
+__device__ inline void load_dims(const T *row, int64_t sd, int d0, int D, float *v) {
     if constexpr (VEC) {
-        struct alignas(16) P {
-            T e[16 / sizeof(T)];
-        };
-        constexpr int PER = 16 / sizeof(T);
-        if (d0 >= D) {  // padding
+        const bool in = d0 < D;  // (else padding)
+        gtvec::Dims16<T> p;
+        p.load(row + (in ? d0 : 0));
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = 0.0f;
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 16 / PER; ++j) {
-            const P p = *(const P *)(row + d0 + j * PER);
-#pragma unroll
-            for (int e = 0; e < PER; ++e) v[j * PER + e] = to_f(p.e[e]);
-        }
+        for (int e = 0; e < 16; ++e) v[e] = in ? p.get(e) : 0.0f;
     } else {
+        T y[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? to_f(row[(int64_t)(d0 + e) * sd]) : 0.0f;
+        for (int e = 0; e < 16; ++e) y[e] = row[(int64_t)min(d0 + e, D - 1) * sd];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? to_f(y[e]) : 0.0f;
     }
 }
 
@@ -62,111 +58,11 @@ __device__ inline uint32_t encode4(float a, float b, float c, float d) {
         w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
         return (uint32_t)w;
     } else {
-        auto q = [](float x) { return (uint32_t)(int)rintf(x) & 0xffu; };
+        // + 128 (kv_blocks.h): the rounded value + 128 is 1 .. 255, whose float32 sum with 2^23 holds it in its low byte
+        auto q = [](float x) { return __float_as_uint(rintf(x) + (8388608.0f + 128.0f)) & 0xffu; };
         return q(a) | q(b) << 8 | q(c) << 16 | q(d) << 24;
     }
 }
-
-struct AppendArgs {
-    const void *src[2];
-    int64_t st[2][4];  // element strides (B, Hkv, T, D)
-    uint8_t *codes[2];
-    float *scales[2], *tail[2];
-    const int32_t *pos;    // tokens held before, per sequence; null: none
-    const int32_t *count;  // tokens appended, per sequence; null: T
-    int32_t *pos_next;     // tokens held afterwards, or null
-    int T, Hkv, N, D, Dp;
-    int64_t units;         // of 64 tokens per sequence and head
-};
-
-// grid: (blocks that an append can fill, at least 1, B * Hkv, K and V)
-template <typename T, bool E4M3, bool VEC>
-__global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a) {
-    const int z = blockIdx.z, N = a.N, D = a.D, Dp = a.Dp, tid = threadIdx.x;
-    const int64_t bg = blockIdx.y, b = bg / a.Hkv, g = bg - b * a.Hkv;
-    const int held = a.pos ? a.pos[b] : 0, more = a.count ? a.count[b] : a.T;
-    const int first = held / N, whole = (held + more) / N;  // whole: blocks full afterwards
-    const int blk = first + (int)blockIdx.x;
-    const T *src = (const T *)a.src[z] + b * a.st[z][0] + g * a.st[z][1];
-    float *tail = a.tail[z] + bg * N * D;
-    __shared__ float s_max[kThreads / 64];
-    if (a.pos_next && tid == 0 && g == 0 && z == 0 && blockIdx.x == 0) a.pos_next[b] = held + more;
-
-    // 16 dims from d0 on of the block's token t: from the tail, where they have been waiting, or from the source
-    auto load = [&](int t, int d0, float *v) {
-        const int p = blk * N + t;
-        if (p < held) {
-            const float *row = tail + (int64_t)t * D;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? row[d0 + e] : 0.0f;
-        } else {
-            load16<T, VEC>(src + (int64_t)(p - held) * a.st[z][2], a.st[z][3], d0, D, v);
-        }
-    };
-    const int chunks = Dp / 16;
-    if (blk < whole) {
-        float amax = 0.0f;
-        bool odd = false;  // an infinity or NaN among them
-        for (int i = tid; i < N * chunks; i += kThreads) {
-            float v[16];
-            load(i / chunks, i % chunks * 16, v);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                amax = fmaxf(amax, fabsf(v[e]));
-                odd = odd || !(fabsf(v[e]) < INFINITY);
-            }
-        }
-        amax = odd ? INFINITY : amax;
-        for (int m = 32; m >= 1; m >>= 1) amax = fmaxf(amax, __shfl_xor(amax, m, 64));
-        if ((tid & 63) == 0) s_max[tid >> 6] = amax;
-        __syncthreads();
-        amax = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
-        const bool bad = amax == INFINITY;
-        const int e2 = bad ? 0 : scale_exponent(__float_as_uint(amax), E4M3);
-        // (a block with an infinity or NaN has no scale: all of it reads as NaN)
-        if (tid == 0) a.scales[z][bg * (a.units * kUnit / N) + blk] = bad ? NAN : __uint_as_float((uint32_t)(e2 + 127) << 23);
-        const float inv = bad ? 0.0f : __uint_as_float((uint32_t)(127 - e2) << 23);
-        uint8_t *codes = a.codes[z] + bg * a.units * kUnit * Dp;
-        if (z == 0) {
-            for (int i = tid; i < N * chunks; i += kThreads) {
-                // 16 threads next to each other write the 16 tokens of a tile's chunk
-                const int t = (i / (16 * chunks)) * 16 + (i & 15), c = (i / 16) % chunks;
-                float v[16];
-                load(t, 16 * c, v);
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w[j] = bad ? 0u : encode4<E4M3>(v[4 * j] * inv, v[4 * j + 1] * inv, v[4 * j + 2] * inv, v[4 * j + 3] * inv);
-                *(uint4 *)(codes + k_at((int64_t)blk * N + t, 16 * c, Dp)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        } else {
-            // a dim of four tokens is four bytes in a row
-            for (int i = tid; i < N / 4 * Dp; i += kThreads) {
-                const int d = i % Dp, t = i / Dp * 4;
-                float v[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int p = blk * N + t + j;
-                    v[j] = d >= D ? 0.0f
-                           : p < held ? tail[(int64_t)(t + j) * D + d]
-                                      : to_f(src[(int64_t)(p - held) * a.st[z][2] + (int64_t)d * a.st[z][3]]);
-                }
-                const uint32_t w = bad ? 0u : encode4<E4M3>(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-                *(uint32_t *)(codes + v_at((int64_t)blk * N + t, d, Dp)) = w;
-            }
-        }
-    }
-    if (blockIdx.x != 0) return;
-    // the tokens after the last whole block; the old tail has been read above
-    __syncthreads();
-    const int from = max(held, whole * N), rows = held + more - from;
-    for (int i = tid; i < rows * D; i += kThreads) {
-        const int r = i / D, d = i - r * D;
-        tail[(int64_t)(from - whole * N + r) * D + d] = to_f(src[(int64_t)(from + r - held) * a.st[z][2] + (int64_t)d * a.st[z][3]]);
-    }
-}
-
-// 8 codes as values.
 template <bool E4M3>
 __device__ inline void decode4(uint32_t w, float *v) {
     if constexpr (E4M3) {
@@ -176,8 +72,330 @@ __device__ inline void decode4(uint32_t w, float *v) {
         v[3] = __builtin_amdgcn_cvt_f32_fp8(w, 3);
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = (float)(int8_t)(w >> (8 * j));
+        for (int j = 0; j < 4; ++j) v[j] = (float)((int)(w >> (8 * j) & 0xffu) - 128);
     }
+}
+
+// One tensor (K or V) of the cache: the codes, scales, tail and the tail's operands.
+struct Side {
+    uint8_t *codes;
+    float *scales, *tail;
+    _Float16 *ops;
+    float *op_scales;
+};
+
+struct AppendArgs {
+    Side to[2];
+    int T, Hkv, N, D;
+    int64_t units;         // of 64 tokens per sequence and head
+    // rows: `T` after the pos[b] tokens held before
+    const void *src[2];
+    int64_t st[2][4];      // element strides (B, Hkv, T, D)
+    const int32_t *pos;
+    int32_t *pos_next;     // tokens held afterwards
+    // eviction: the kept[b, g, 0 .. min(len[b], keep) - 1] of another cache, into an empty one
+    Side from[2];
+    const int32_t *len;
+    const int64_t *kept;
+    int keep;
+};
+
+// Where an append's tokens come from.  dims: 16 dims of token p from d0 on; column: dim d (< D) of the tokens p(0)
+// .. p(15), the same for a whole wavefront (their addresses are scalar), of which there(i) tells whether it is
+// wanted.
+template <typename T, bool VEC>
+struct RowSource {
+    const T *rows;
+    int64_t sr, sd;
+    const float *tail;
+    int held, blk0, D;  // blk0: the tail's first token
+    __device__ void dims(int p, int d0, float *v) const {
+        load_dims<T, VEC>(rows + (int64_t)max(p - held, 0) * sr, sd, d0, D, v);
+        if (p < held) {  // waiting in the tail
+            const float *row = tail + (int64_t)(p - blk0) * D;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? row[d0 + e] : 0.0f;
+        }
+    }
+    template <typename P, typename W>
+    __device__ void column(P &&p, W &&there, int d, float *v) const {
+        T y[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const T *row = rows + (int64_t)(there(i) ? max(p(i) - held, 0) : 0) * sr;
+            y[i] = row[d * (int)sd];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = to_f(y[i]);
+        if (p(0) < held) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (there(i) && p(i) < held) v[i] = tail[(int64_t)(p(i) - blk0) * D + d];
+        }
+    }
+};
+
+// Tokens of another block cache (z 0 keys, 1 values): kept[0 .. count - 1], in LDS.
+template <bool E4M3>
+struct KeptSource {
+    const uint8_t *codes;
+    const float *scales, *tail;
+    const int *kept;
+    int first, full, N, D, Dp, z;  // kept[0] is token `first` of the new cache
+    __device__ void dims(int p, int d0, float *v) const {
+        const int t = kept[p - first];
+        if (t >= full) {
+            const float *row = tail + (int64_t)(t - full) * D;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? row[d0 + e] : 0.0f;
+            return;
+        }
+        const float s = scales[t / N];
+        if (z == 0) {
+            const uint4 w = *(const uint4 *)(codes + k_at(t, d0, Dp));
+            decode4<E4M3>(w.x, v);
+            decode4<E4M3>(w.y, v + 4);
+            decode4<E4M3>(w.z, v + 8);
+            decode4<E4M3>(w.w, v + 12);
+        } else {
+            const uint8_t *q = codes + v_at(t, d0, Dp);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                decode4<E4M3>(q[64 * j] | (uint32_t)q[64 * j + 16] << 8 | (uint32_t)q[64 * j + 32] << 16 | (uint32_t)q[64 * j + 48] << 24, v + 4 * j);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= s;
+    }
+    template <typename P, typename W>
+    __device__ void column(P &&p, W &&there, int d, float *v) const {
+        uint32_t q[16];
+        float s[16];
+        bool late = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = there(i) ? __builtin_amdgcn_readfirstlane(kept[p(i) - first]) : 0;
+            const int tc = t < full ? t : 0;  // (token 0's codes are there to be read)
+            late = late || t >= full;
+            q[i] = (codes + v_at(tc, 0, Dp))[(uint32_t)((d >> 4) * 1024 + (d & 15) * 16)];
+            s[i] = scales[tc / N];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) decode4<E4M3>(q[4 * j] | q[4 * j + 1] << 8 | q[4 * j + 2] << 16 | q[4 * j + 3] << 24, v + 4 * j);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= s[i];
+        if (late) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = there(i) ? __builtin_amdgcn_readfirstlane(kept[p(i) - first]) : 0;
+                if (t >= full) v[i] = tail[(int64_t)(t - full) * D + d];
+            }
+        }
+    }
+};
+
+// NT tokens a workgroup, whole blocks of N.  `held` tokens were there, `total` are there afterwards; the workgroup
+// x of a (sequence, head) takes the x-th NT tokens from those of the block in progress on, t0 the first.
+template <bool E4M3, int DP, int NT, typename Source>
+__device__ inline void append_blocks(const Source &src, const Side &to, int N, int D, int z, int t0, int held, int total) {
+    constexpr int ITEMS = NT * DP / 16 / kThreads, CH = DP / 16, BLOCKS = NT / 32;
+    const int tid = threadIdx.x, lane = tid & 63;
+    __shared__ uint32_t s_max[BLOCKS][kThreads / 64];
+    // a block is written when it becomes full
+    auto fills = [&](int t) { return (t / N + 1) * N > held && (t / N + 1) * N <= total; };
+    // item i of a thread.  K: dims 16 ch .. of token t, 16 lanes next to each other the 16 tokens of a tile, whose
+    // chunk is contiguous in the codes.  V: the 16 tokens 16 kb + 4g + r of dim d, contiguous in the codes as well.
+    auto k_token = [&](int i) { return t0 + i / (16 * CH) * 16 + (i & 15); };
+    auto k_dim = [&](int i) { return i / 16 % CH * 16; };
+    // + 16 kb + r; the same for the 64 threads of a wavefront
+    auto v_unit = [&](int i) { return __builtin_amdgcn_readfirstlane(t0 + i / (4 * DP) * kUnit + 4 * (i / DP % 4)); };
+    float x[ITEMS][16];
+    // magnitudes as their bits, whose order is theirs, NaN above infinity
+    uint32_t amax[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) amax[b] = 0;
+    auto magnitude = [&](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        const int i = tid + kThreads * it;
+        if (z == 0) {
+            const int t = k_token(i);
+            if (!fills(t)) continue;
+            src.dims(t, k_dim(i), x[it]);
+            uint32_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = max(most, magnitude(x[it][e]));
+#pragma unroll
+            for (int b = 0; b < BLOCKS; ++b) amax[b] = b == (t - t0) / N ? max(amax[b], most) : amax[b];
+        } else {
+            const int t = v_unit(i), d = i % DP;
+            if (!fills(t) && !fills(t + 32)) continue;
+            if (d < D) {
+                src.column([&](int e) { return t + 16 * (e >> 2) + (e & 3); }, [&](int e) { return fills(t + 16 * (e >> 2)); }, d, x[it]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[it][e] = 0.0f;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!fills(t + 32 * h)) continue;
+                uint32_t most = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = max(most, magnitude(x[it][8 * h + e]));
+#pragma unroll
+                for (int b = 0; b < BLOCKS; ++b) amax[b] = b == (t + 32 * h - t0) / N ? max(amax[b], most) : amax[b];
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        for (int m = 32; m >= 1; m >>= 1) amax[b] = max(amax[b], (uint32_t)__shfl_xor((int)amax[b], m, 64));
+        if (lane == 0) s_max[b][tid >> 6] = amax[b];
+    }
+    __syncthreads();
+    float inv[BLOCKS];
+#pragma unroll
+    for (int b = 0; b < BLOCKS; ++b) {
+        const uint32_t most = max(max(s_max[b][0], s_max[b][1]), max(s_max[b][2], s_max[b][3]));
+        const bool bad = most >= 0x7f800000u;
+        const int e2 = bad ? 0 : scale_exponent(most, E4M3);
+        // (a block with an infinity or NaN has no scale: all of it reads as NaN)
+        inv[b] = bad ? NAN : __uint_as_float((uint32_t)(127 - e2) << 23);
+        if (tid == 0 && b * N < NT && fills(t0 + b * N))
+            to.scales[t0 / N + b] = bad ? NAN : __uint_as_float((uint32_t)(e2 + 127) << 23);
+    }
+    auto inv_of = [&](int t) {
+        float f = 0.0f;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b) f = b == (t - t0) / N ? inv[b] : f;
+        return f;
+    };
+    auto encode = [&](const float *v, float f) {
+        return f != f ? (E4M3 ? 0u : 0x80808080u) : encode4<E4M3>(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+    };
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+        const int i = tid + kThreads * it;
+        if (z == 0) {
+            const int t = k_token(i);
+            if (!fills(t)) continue;
+            const float f = inv_of(t);
+            *(uint4 *)(to.codes + k_at(t, k_dim(i), DP)) = make_uint4(encode(x[it], f), encode(x[it] + 4, f), encode(x[it] + 8, f), encode(x[it] + 12, f));
+        } else {
+            const int t = v_unit(i), d = i % DP;
+            uint2 *o = (uint2 *)(to.codes + v_at(t, d, DP));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (!fills(t + 32 * h)) {
+                    // the unit's other block, of tokens to come: the attention reads it, with weights of 0, so it must not
+                    // be e4m3 NaNs
+                    if (h == 1 && t + 32 >= total / N * N) o[1] = make_uint2(0u, 0u);
+                    continue;
+                }
+                const float f = inv_of(t + 32 * h);
+                o[h] = make_uint2(encode(x[it] + 8 * h, f), encode(x[it] + 8 * h + 4, f));
+            }
+        }
+    }
+}
+
+// The tokens after the last whole block, from token `from` of the cache on (those before are there): their values,
+// and the operands that the attention takes them as (the row divided by its own power of two, float16 hi + lo, in
+// the codes' order), DP / 16 lanes a row.  clear: zero operands behind them.
+template <int DP, typename Source>
+__device__ inline void append_tail(const Source &src, const Side &to, int N, int D, int z, int from, int total, bool clear) {
+    constexpr int CH = DP / 16;
+    const int whole = total / N * N, room = max(N, kUnit), rows = clear ? room - (from - whole) : total - from;
+    for (int i = threadIdx.x; i < rows * CH; i += kThreads) {
+        const int p = from + i / CH, t = p - whole, d0 = i % CH * 16;
+        float v[16];
+        if (p < total) src.dims(p, d0, v);
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            v[e] = p < total ? v[e] : 0.0f;
+            most = fmaxf(most, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : INFINITY);
+        }
+        for (int m = CH / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
+        const bool bad = most == INFINITY;
+        const int e2 = bad || most == 0.0f ? -126 : min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+        const float f = __uint_as_float((uint32_t)(127 - e2) << 23);
+        if (d0 == 0) to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
+        if (p < total) {
+            float *row = to.tail + (int64_t)t * D;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (d0 + e < D) row[d0 + e] = v[e];
+        }
+        _Float16 hi[16], lo[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float y = bad ? 0.0f : v[e] * f;
+            hi[e] = (_Float16)y;
+            lo[e] = (_Float16)(y - (float)hi[e]);
+        }
+        const int64_t plane = (int64_t)room * DP;
+        if (z == 0) {
+            struct alignas(16) P {
+                _Float16 e[16];
+            };
+            *(P *)(to.ops + k_at(t, d0, DP)) = *(const P *)hi;
+            *(P *)(to.ops + plane + k_at(t, d0, DP)) = *(const P *)lo;
+        } else {
+            _Float16 *o = to.ops + v_at(t, d0, DP);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                o[16 * e] = hi[e];
+                o[plane + 16 * e] = lo[e];
+            }
+        }
+    }
+}
+
+template <int DP>
+__device__ inline Side slice(const Side &s, const AppendArgs &a, int64_t bg) {
+    Side r;
+    r.codes = s.codes + bg * a.units * kUnit * DP;
+    r.scales = s.scales + bg * (a.units * kUnit / a.N);
+    r.tail = s.tail + bg * a.N * a.D;
+    r.ops = s.ops + bg * 2 * max(a.N, kUnit) * DP;
+    r.op_scales = s.op_scales + bg * max(a.N, kUnit);
+    return r;
+}
+
+// grid: (NT tokens each, B * Hkv, K and V)
+template <typename T, bool E4M3, bool VEC, int DP, int NT>
+__global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a) {
+    const int z = blockIdx.z;
+    const int64_t bg = blockIdx.y, b = bg / a.Hkv, g = bg - b * a.Hkv;
+    const int held = a.pos[b], total = held + a.T;
+    if (threadIdx.x == 0 && g == 0 && z == 0 && blockIdx.x == 0) a.pos_next[b] = total;
+    const int t0 = (held / NT + (int)blockIdx.x) * NT;
+    const Side to = slice<DP>(a.to[z], a, bg);
+    const RowSource<T, VEC> src = {(const T *)a.src[z] + b * a.st[z][0] + g * a.st[z][1], a.st[z][2], a.st[z][3], to.tail,
+                                   held, held / a.N * a.N, a.D};
+    // (a decode step that fills no block has none to look at)
+    if (held / a.N != total / a.N) append_blocks<E4M3, DP, NT>(src, to, a.N, a.D, z, t0, held, total);
+    // by the workgroup that has read the old tail
+    if (blockIdx.x != 0) return;
+    __syncthreads();
+    append_tail<DP>(src, to, a.N, a.D, z, max(held, total / a.N * a.N), total, false);
+}
+
+template <bool E4M3, int DP, int NT>
+__global__ __launch_bounds__(kThreads) void kv_blocks_evict_kernel(AppendArgs a) {
+    __shared__ int s_kept[NT];
+    const int z = blockIdx.z;
+    const int64_t bg = blockIdx.y, b = bg / a.Hkv;
+    const int total = min(a.len[b], a.keep), t0 = (int)blockIdx.x * NT;
+    if (t0 >= total && (int)blockIdx.x > 0) return;  // (an empty sequence: its operands are cleared)
+    for (int i = threadIdx.x; i < min(NT, total - t0); i += kThreads) s_kept[i] = (int)a.kept[bg * a.keep + t0 + i];
+    __syncthreads();
+    const Side from = slice<DP>(a.from[z], a, bg), to = slice<DP>(a.to[z], a, bg);
+    const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, a.len[b] / a.N * a.N, a.N, a.D, DP, z};
+    append_blocks<E4M3, DP, NT>(src, to, a.N, a.D, z, t0, 0, total);
+    const int whole = total / a.N * a.N;
+    // the tail's tokens are among the last workgroup's, or there are none
+    if (total - t0 <= NT) append_tail<DP>(src, to, a.N, a.D, z, whole, total, true);
 }
 
 struct ReadArgs {
@@ -185,15 +403,17 @@ struct ReadArgs {
     const float *scales[2], *tail[2];
     void *out[2];            // dense (B, Hkv, rows, D)
     const int32_t *len;      // tokens held per sequence
-    const int64_t *kept;     // (B, Hkv, rows) tokens to read, or null: 0, 1, ...
     int rows, Hkv, N, D, Dp;
     int64_t units;
 };
 
 // grid: (units of 64 rows, B * Hkv, K and V); rows past what is held are zero
-template <typename TO, bool E4M3, bool GATHER>
+template <typename TO, bool E4M3>
 __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
-    __shared__ __attribute__((aligned(16))) uint8_t raw[GATHER ? 16 : kUnit * kMaxDim];
+    // (K: a chunk of 16 dims at a pitch of 64 more bytes a tile, V: 16 dims at one of 16 more a unit, so that the lanes
+    // of a row, 8 dims each, read from different banks)
+    constexpr int KP = 256 + 64, VP = 1024 + 16;
+    __shared__ __attribute__((aligned(16))) uint8_t raw[kMaxDim / 16 * 4 * KP];
     const int z = blockIdx.z, N = a.N, D = a.D, Dp = a.Dp, tid = threadIdx.x;
     const int64_t bg = blockIdx.y, b = bg / a.Hkv;
     const int r0 = blockIdx.x * kUnit, held = a.len[b], full = held / N * N;
@@ -201,36 +421,31 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
     const float *scales = a.scales[z] + bg * (a.units * kUnit / N);
     const float *tail = a.tail[z] + bg * N * D;
     TO *out = (TO *)a.out[z] + bg * (int64_t)a.rows * D;
-    if constexpr (!GATHER) {
-        if (r0 < full) {
-            for (int i = tid; i < kUnit * Dp / 16; i += kThreads)
-                *(uint4 *)(raw + 16 * i) = *(const uint4 *)(codes + (int64_t)r0 * Dp + 16 * i);
-        }
-        __syncthreads();
+    if (r0 < full) {
+        for (int i = tid; i < kUnit * Dp / 16; i += kThreads)
+            *(uint4 *)(raw + (z == 0 ? i / 16 * KP + i % 16 * 16 : i / 64 * VP + i % 64 * 16)) = *(const uint4 *)(codes + (int64_t)r0 * Dp + 16 * i);
     }
+    __syncthreads();
     const int groups = Dp / 8, n = min(kUnit, a.rows - r0);
     for (int i = tid; i < n * groups; i += kThreads) {
         const int r = i / groups, d0 = i % groups * 8;
         if (d0 >= D) continue;
-        int64_t t = r0 + r;
-        if constexpr (GATHER) t = a.kept[bg * a.rows + t];
+        const int t = r0 + r;
         float v[8];
-        if (t < 0 || t >= held) {
+        if (t >= held) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = 0.0f;
         } else if (t >= full) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = d0 + e < D ? tail[(t - full) * D + d0 + e] : 0.0f;
+            for (int e = 0; e < 8; ++e) v[e] = d0 + e < D ? tail[(int64_t)(t - full) * D + d0 + e] : 0.0f;
         } else {
             uint32_t w[2];
-            const uint8_t *base = GATHER ? codes : raw;
-            const int64_t tt = GATHER ? t : r;
             if (z == 0) {
-                const uint2 q = *(const uint2 *)(base + k_at(tt, d0, Dp));
+                const uint2 q = *(const uint2 *)(raw + ((r >> 4) * (Dp / 16) + (d0 >> 4)) * KP + (r & 15) * 16 + (d0 & 15));
                 w[0] = q.x;
                 w[1] = q.y;
             } else {
-                const uint8_t *p = base + v_at(tt, d0, Dp);
+                const uint8_t *p = raw + (d0 >> 4) * VP + v_at(r, d0 & 15, 16);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
                     w[j] = p[64 * j] | (uint32_t)p[64 * j + 16] << 8 | (uint32_t)p[64 * j + 32] << 16 | (uint32_t)p[64 * j + 48] << 24;
@@ -257,69 +472,89 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
     }
 }
 
+// The kernel for head sizes padded to Dp and blocks of N.
+template <typename T, bool E4M3, bool VEC>
+const void *append_kernel(int Dp, int N) {
+#define GT_A(DP) (N == 128 ? (const void *)kv_blocks_append_kernel<T, E4M3, VEC, DP, 128> : (const void *)kv_blocks_append_kernel<T, E4M3, VEC, DP, 64>)
+    return Dp == 64 ? GT_A(64) : Dp == 128 ? GT_A(128) : GT_A(256);
+#undef GT_A
+}
 template <typename T>
-hipError_t launch_append(const AppendArgs &a, bool e4m3, bool vec, dim3 grid, hipStream_t s) {
-    if (e4m3) {
-        if (vec) hipLaunchKernelGGL((kv_blocks_append_kernel<T, true, true>), grid, dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((kv_blocks_append_kernel<T, true, false>), grid, dim3(kThreads), 0, s, a);
-    } else {
-        if (vec) hipLaunchKernelGGL((kv_blocks_append_kernel<T, false, true>), grid, dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((kv_blocks_append_kernel<T, false, false>), grid, dim3(kThreads), 0, s, a);
-    }
-    return hipGetLastError();
+const void *append_kernel(bool e4m3, bool vec, int Dp, int N) {
+    if (e4m3) return vec ? append_kernel<T, true, true>(Dp, N) : append_kernel<T, true, false>(Dp, N);
+    return vec ? append_kernel<T, false, true>(Dp, N) : append_kernel<T, false, false>(Dp, N);
+}
+template <bool E4M3>
+const void *evict_kernel(int Dp, int N) {
+#define GT_E(DP) (N == 128 ? (const void *)kv_blocks_evict_kernel<E4M3, DP, 128> : (const void *)kv_blocks_evict_kernel<E4M3, DP, 64>)
+    return Dp == 64 ? GT_E(64) : Dp == 128 ? GT_E(128) : GT_E(256);
+#undef GT_E
+}
+
+void fill_sides(Side *s, const gt_kv_blocks &c) {
+    for (int z = 0; z < 2; ++z) s[z] = {(uint8_t *)c.codes[z], c.scales[z], c.tail[z], (_Float16 *)c.ops[z], c.op_scales[z]};
+}
+
+hipError_t launch(const void *kernel, AppendArgs &a, int64_t groups, int64_t bg, hipStream_t s) {
+    if (bg > 65535 || groups > 0x7fffffff) return hipErrorInvalidConfiguration;
+    void *args[] = {(void *)&a};
+    return hipLaunchKernel(kernel, dim3((unsigned)std::max<int64_t>(groups, 1), (unsigned)bg, 2), dim3(kThreads), args, 0, s);
 }
 
 template <typename TO>
 hipError_t launch_read(const ReadArgs &a, bool e4m3, dim3 grid, hipStream_t s) {
-    if (a.kept) {
-        if (e4m3) hipLaunchKernelGGL((kv_blocks_read_kernel<TO, true, true>), grid, dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((kv_blocks_read_kernel<TO, false, true>), grid, dim3(kThreads), 0, s, a);
-    } else {
-        if (e4m3) hipLaunchKernelGGL((kv_blocks_read_kernel<TO, true, false>), grid, dim3(kThreads), 0, s, a);
-        else hipLaunchKernelGGL((kv_blocks_read_kernel<TO, false, false>), grid, dim3(kThreads), 0, s, a);
-    }
+    if (e4m3) hipLaunchKernelGGL((kv_blocks_read_kernel<TO, true>), grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((kv_blocks_read_kernel<TO, false>), grid, dim3(kThreads), 0, s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t gt_launch_kv_blocks_append(const gt_kv_blocks &c, const void *const *src, int src_dtype,
-                                      const int64_t *const *strides, const int32_t *pos, const int32_t *count,
-                                      int32_t *pos_next, int64_t T, int64_t blocks, hipStream_t s) {
+                                      const int64_t *const *strides, const int32_t *pos, int32_t *pos_next, int64_t T,
+                                      int64_t groups, hipStream_t s) {
     AppendArgs a{};
     bool vec = c.D % 16 == 0;
     const int64_t es = src_dtype == GT_F32 ? 4 : 2;
     for (int z = 0; z < 2; ++z) {
         a.src[z] = src[z];
         for (int i = 0; i < 4; ++i) a.st[z][i] = strides[z][i];
-        a.codes[z] = (uint8_t *)c.codes[z];
-        a.scales[z] = c.scales[z];
-        a.tail[z] = c.tail[z];
         vec = vec && strides[z][3] == 1 && (uintptr_t)src[z] % 16 == 0;
         for (int i = 0; i < 3; ++i) vec = vec && strides[z][i] * es % 16 == 0;
     }
+    fill_sides(a.to, c);
     a.pos = pos;
-    a.count = count;
     a.pos_next = pos_next;
     a.T = (int)T;
     a.Hkv = (int)c.Hkv;
     a.N = c.N;
     a.D = (int)c.D;
-    a.Dp = c.Dp;
     a.units = c.units;
-    const int64_t bg = c.B * c.Hkv;
-    if (bg > 65535 || blocks > 0x7fffffff) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)std::max<int64_t>(blocks, 1), (unsigned)bg, 2);
-    switch (src_dtype) {
-        case GT_F32: return launch_append<float>(a, c.e4m3, vec, grid, s);
-        case GT_F16: return launch_append<_Float16>(a, c.e4m3, vec, grid, s);
-        case GT_BF16: return launch_append<__bf16>(a, c.e4m3, vec, grid, s);
-        default: return hipErrorInvalidValue;
-    }
+    const void *kernel = src_dtype == GT_F32   ? append_kernel<float>(c.e4m3, vec, c.Dp, c.N)
+                         : src_dtype == GT_F16 ? append_kernel<_Float16>(c.e4m3, vec, c.Dp, c.N)
+                                               : append_kernel<__bf16>(c.e4m3, vec, c.Dp, c.N);
+    return launch(kernel, a, groups, c.B * c.Hkv, s);
 }
 
-hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, const int64_t *kept, int64_t rows,
-                                    void *k, void *v, int dtype, hipStream_t s) {
+hipError_t gt_launch_kv_blocks_evict(const gt_kv_blocks &from, const gt_kv_blocks &to, const int32_t *len, const int64_t *kept,
+                                     int64_t keep, hipStream_t s) {
+    AppendArgs a{};
+    fill_sides(a.to, to);
+    fill_sides(a.from, from);
+    a.len = len;
+    a.kept = kept;
+    a.keep = (int)keep;
+    a.Hkv = (int)from.Hkv;
+    a.N = from.N;
+    a.D = (int)from.D;
+    a.units = from.units;
+    const int64_t nt = std::max(from.N, kUnit);
+    return launch(from.e4m3 ? evict_kernel<true>(from.Dp, from.N) : evict_kernel<false>(from.Dp, from.N), a, (keep + nt - 1) / nt,
+                  from.B * from.Hkv, s);
+}
+
+hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, int64_t rows, void *k, void *v, int dtype,
+                                    hipStream_t s) {
     if (rows <= 0) return hipSuccess;
     ReadArgs a{};
     for (int z = 0; z < 2; ++z) {
@@ -330,7 +565,6 @@ hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, c
     a.out[0] = k;
     a.out[1] = v;
     a.len = len;
-    a.kept = kept;
     a.rows = (int)rows;
     a.Hkv = (int)c.Hkv;
     a.N = c.N;

@@ -29,6 +29,8 @@ struct SelectArgs {
     const float *w;
     int64_t wb, wg, ws;  // element strides of the weights
     const int32_t *len;
+    int32_t *next;       // the lengths afterwards
+    int32_t *evicted;    // tokens evicted so far, or null (none are)
     int64_t *kept;       // (B, Hkv, keep)
     int Hkv, keep, recent;
 };
@@ -42,6 +44,10 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a)
     const int64_t bg = blockIdx.x, b = bg / a.Hkv, g = bg - b * a.Hkv;
     const int n = a.len[b];
     int64_t *kept = a.kept + bg * a.keep;
+    if (g == 0 && tid == 0) {
+        a.next[b] = min(n, a.keep);
+        if (n > a.keep) a.evicted[b] += n - a.keep;
+    }
     if (n <= a.keep) {
         for (int i = tid; i < a.keep; i += kSelectThreads) kept[i] = i < n ? i : -1;
         return;
@@ -115,15 +121,6 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a)
         if (up || (eq && pe < (int)need)) kept[pu + min(pe, (int)need)] = i;
         __syncthreads();
     }
-}
-
-// count[b]: the tokens that a sequence's cache is rewritten with (0: it loses none); next[b]: its tokens then.
-__global__ void kv_evict_lengths_kernel(const int32_t *len, int32_t *next, int32_t *count, int keep, int B) {
-    const int b = blockIdx.x * blockDim.x + threadIdx.x;
-    if (b >= B) return;
-    const int n = len[b];
-    next[b] = min(n, keep);
-    count[b] = n > keep ? keep : 0;
 }
 
 struct MoveArgs {
@@ -217,16 +214,11 @@ hipError_t launch_rows_read(const void *k, const void *v, const int32_t *len, vo
 
 }  // namespace
 
-hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int64_t *kept, int64_t B, int64_t Hkv,
-                               int64_t keep, int64_t recent, hipStream_t s) {
-    SelectArgs a{w, strides[0], strides[1], strides[2], len, kept, (int)Hkv, (int)keep, (int)recent};
+hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int32_t *next, int32_t *evicted, int64_t *kept,
+                               int64_t B, int64_t Hkv, int64_t keep, int64_t recent, hipStream_t s) {
+    SelectArgs a{w, strides[0], strides[1], strides[2], len, next, evicted, kept, (int)Hkv, (int)keep, (int)recent};
     if (B * Hkv > 0x7fffffff) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)(B * Hkv)), dim3(kSelectThreads), 0, s, a);
-    return hipGetLastError();
-}
-
-hipError_t gt_launch_kv_evict_lengths(const int32_t *len, int32_t *next, int32_t *count, int64_t keep, int64_t B, hipStream_t s) {
-    hipLaunchKernelGGL(kv_evict_lengths_kernel, dim3((unsigned)((B + 255) / 256)), dim3(256), 0, s, len, next, count, (int)keep, (int)B);
     return hipGetLastError();
 }
 
