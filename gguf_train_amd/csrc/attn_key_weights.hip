@@ -31,7 +31,7 @@ struct Args {
     const float *ks;       // a block cache's scales, and its tail's operands and scales
     const _Float16 *kt;
     const float *kts;
-    int N;
+    int shift;  // log2 of the tokens of a block
     int64_t units;
     const float *lse;
     const int32_t *len;
@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t bg = blockIdx.y, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
-    const int len = a.len[b], full = CODES ? len / a.N * a.N : 0;
+    const int len = a.len[b], full = CODES ? len >> a.shift << a.shift : 0;
     const int k0 = ((int)blockIdx.x * kWaves + w) * 16 * TW;
     if (k0 >= len) return;
 
@@ -163,12 +163,12 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
                     kl[kb][i][j] = half8{0, 0, 0, 0, 0, 0, 0, 0};
                 }
             }
-            const float s = a.ks[bg * (a.units * kUnit / a.N) + t0 / a.N];
+            const float s = a.ks[bg * (a.units * kUnit >> a.shift) + (t0 >> a.shift)];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = s;
         } else if constexpr (CODES) {
             lo_used = true;
-            const int room = max(a.N, kUnit), at = min(t0 - full, room - 16);  // (the last tiles may hold no token)
+            const int room = max(1 << a.shift, kUnit), at = min(t0 - full, room - 16);  // (the last tiles may hold no token)
             const _Float16 *p = a.kt + (bg * 2 * room + at) * Dp + 16 * lane;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
@@ -300,7 +300,7 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
         a.ks = r.blocks->scales[0];
         a.kt = (const _Float16 *)r.blocks->ops[0];
         a.kts = r.blocks->op_scales[0];
-        a.N = r.blocks->N;
+        a.shift = r.blocks->N == 32 ? 5 : r.blocks->N == 64 ? 6 : 7;
         a.units = r.blocks->units;
     } else {
         src = r.k_dtype == GT_F16 ? kF16 : r.k_dtype == GT_BF16 ? kBf16 : r.k_dtype == GT_F32 ? kF32 : kQ8;

@@ -63,7 +63,8 @@ struct AttnArgs {
     const int32_t *len;
     float scale;
     int causal, q_vec;  // q_vec: query rows in aligned 16-byte pieces, D a multiple of 16
-    int B, H, Hkv, L, D, N;
+    int B, H, Hkv, L, D;
+    int shift;  // log2 of the tokens of a block
     int64_t units;  // of a slice
     int groups;     // row groups per kv head
     int nsplit, span;  // splits, units of each
@@ -244,7 +245,7 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     const int64_t x = blockIdx.x, bg = x / a.groups, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
     const int rg = (int)(x - bg * a.groups), G = a.H / a.Hkv, rows = G * a.L;
     const int r0 = rg * COLS, nr = min(COLS, rows - r0);
-    const int len = a.len[b], full = len / a.N * a.N, tail = len - full;
+    const int len = a.len[b], full = len >> a.shift << a.shift, tail = len - full;
 
     // queries, and the first key that each column does not see
     half8 qh[CT][NI][2], ql[CT][NI][2];
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     const int bytes = max(u1 - u0, 0) * kUnit * Dp;  // (below 2^31: gt_kv_blocks_attn_supported)
     const auto kr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + from), 0, bytes, 0x00027000);
     const auto vr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + from), 0, bytes, 0x00027000);
-    const int64_t nblk = a.units * kUnit / a.N;
+    const int64_t nblk = a.units * kUnit >> a.shift;
     const float *sc = ((lane & 4) ? a.vs : a.ks) + bg * nblk;  // lanes 0..3 hold K's scales, 4..7 V's
     u32x4 rk[DT], rv[DT];
     float rs = 0.0f;
@@ -351,7 +352,7 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
 #pragma unroll
         for (int t = 0; t < DT; ++t)
             rk[t] = __builtin_amdgcn_raw_buffer_load_b128(kr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
-        rs = sc[min((int64_t)(u * kUnit + 16 * (lane & 3)) / a.N, nblk - 1)];
+        rs = sc[min((u * kUnit + 16 * (lane & 3)) >> a.shift, (int)nblk - 1)];
     };
     auto load_v = [&](int u) {
 #pragma unroll
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     // ---- the tail: by the last split that has units, as its next ones ----
     const int nu = max(u1 - u0, 0);
     const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && u1 * kUnit >= full;
-    const int room = max(a.N, kUnit);  // tokens of a plane of operands
+    const int room = max(1 << a.shift, kUnit);  // tokens of a plane of operands
     for (int tu = 0; mine && tu * kUnit < tail; ++tu) {
         if ((nu + tu) % kWaves != w) continue;
         const int t0 = tu * kUnit;

@@ -67,7 +67,7 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
     a.Hkv = (int)c.Hkv;
     a.L = (int)r.L;
     a.D = (int)c.D;
-    a.N = c.N;
+    a.shift = c.N == 32 ? 5 : c.N == 64 ? 6 : 7;
     a.units = c.units;
     // columns of a workgroup: the fewest that hold the rows, as many as the head size allows
     const int64_t rows = r.H / c.Hkv * r.L;

@@ -31,25 +31,6 @@ __device__ inline T from_f(float x) {
     return (T)x;
 }
 
-// 16 dims of a row from d0 on as float32, zeros from D on; VEC: contiguous, 16-byte aligned, D % 16 == 0.  (No
-// branch around a load: several are in flight.)
-template <typename T, bool VEC>
-__device__ inline void load_dims(const T *row, int64_t sd, int d0, int D, float *v) {
-    if constexpr (VEC) {
-        const bool in = d0 < D;  // (else padding)
-        gtvec::Dims16<T> p;
-        p.load(row + (in ? d0 : 0));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = in ? p.get(e) : 0.0f;
-    } else {
-        T y[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = row[(int64_t)min(d0 + e, D - 1) * sd];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? to_f(y[e]) : 0.0f;
-    }
-}
-
 // Four values already divided by the scale, as codes (round to nearest even).
 template <bool E4M3>
 __device__ inline uint32_t encode4(float a, float b, float c, float d) {
@@ -86,7 +67,8 @@ struct Side {
 
 struct AppendArgs {
     Side to[2];
-    int T, Hkv, N, D;
+    int T, Hkv, D;
+    int shift;             // log2 of the tokens of a block
     int64_t units;         // of 64 tokens per sequence and head
     // rows: `T` after the pos[b] tokens held before
     const void *src[2];
@@ -100,94 +82,125 @@ struct AppendArgs {
     int keep;
 };
 
-// Where an append's tokens come from.  dims: 16 dims of token p from d0 on; column: dim d (< D) of the tokens p(0)
-// .. p(15), the same for a whole wavefront (their addresses are scalar), of which there(i) tells whether it is
-// wanted.
+// Where an append's tokens come from, in two steps, so that all of a thread's loads are in flight together: no branch
+// around a load (a token that is not wanted is read at a place that is there), and the values afterwards.
+//   Dims: 16 dims of token p from d0 on, zeros from D on;
+//   Column: dim d (below the padded size; zeros from D on) of the tokens t + 16 (e / 4) + e % 4, e < 16, t the same
+//   for a whole wavefront (their addresses are scalar).
 template <typename T, bool VEC>
 struct RowSource {
     const T *rows;
     int64_t sr, sd;
     const float *tail;
-    int held, blk0, D;  // blk0: the tail's first token
-    __device__ void dims(int p, int d0, float *v) const {
-        load_dims<T, VEC>(rows + (int64_t)max(p - held, 0) * sr, sd, d0, D, v);
-        if (p < held) {  // waiting in the tail
-            const float *row = tail + (int64_t)(p - blk0) * D;
+    int held, count, blk0, D;  // blk0: the tail's first token
+    struct Dims {
+        gtvec::Dims16<T> w;
+        T y[VEC ? 1 : 16];
+    };
+    struct Column {
+        T y[16];
+    };
+    __device__ const T *row(int p) const { return rows + (int64_t)min(max(p - held, 0), count - 1) * sr; }
+    __device__ void load(Dims &r, int p, int d0) const {
+        if constexpr (VEC) {  // contiguous dims, 16-byte aligned rows, D a multiple of 16
+            r.w.load(row(p) + (d0 < D ? d0 : 0));
+        } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? row[d0 + e] : 0.0f;
+            for (int e = 0; e < 16; ++e) r.y[e] = row(p)[(int64_t)min(d0 + e, D - 1) * sd];
         }
     }
-    template <typename P, typename W>
-    __device__ void column(P &&p, W &&there, int d, float *v) const {
-        T y[16];
+    __device__ void values(const Dims &r, int p, int d0, float *v) const {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const T *row = rows + (int64_t)(there(i) ? max(p(i) - held, 0) : 0) * sr;
-            y[i] = row[d * (int)sd];
+        for (int e = 0; e < 16; ++e) {
+            float x;
+            if constexpr (VEC) x = r.w.get(e);
+            else x = to_f(r.y[e]);
+            v[e] = (VEC ? d0 : d0 + e) < D ? x : 0.0f;
         }
+        if (p < held) {  // waiting in the tail
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = to_f(y[i]);
-        if (p(0) < held) {
+            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? tail[(int64_t)(p - blk0) * D + d0 + e] : 0.0f;
+        }
+    }
+    __device__ void load(Column &r, int t, int d) const {
+        const int at = min(d, D - 1) * (int)sd;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (there(i) && p(i) < held) v[i] = tail[(int64_t)(p(i) - blk0) * D + d];
+        for (int e = 0; e < 16; ++e) r.y[e] = row(t + 16 * (e >> 2) + (e & 3))[at];
+    }
+    __device__ void values(const Column &r, int t, int d, float *v) const {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = d < D ? to_f(r.y[e]) : 0.0f;
+        if (t < held) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int p = t + 16 * (e >> 2) + (e & 3);
+                if (p >= blk0 && p < held) v[e] = d < D ? tail[(int64_t)(p - blk0) * D + d] : 0.0f;
+            }
         }
     }
 };
 
-// Tokens of another block cache (z 0 keys, 1 values): kept[0 .. count - 1], in LDS.
+// Tokens of another block cache (z 0 keys, 1 values): token `first` + i of the new cache is kept[i], in LDS.
 template <bool E4M3>
 struct KeptSource {
     const uint8_t *codes;
     const float *scales, *tail;
     const int *kept;
-    int first, full, N, D, Dp, z;  // kept[0] is token `first` of the new cache
-    __device__ void dims(int p, int d0, float *v) const {
-        const int t = kept[p - first];
-        if (t >= full) {
-            const float *row = tail + (int64_t)(t - full) * D;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? row[d0 + e] : 0.0f;
-            return;
-        }
-        const float s = scales[t / N];
-        if (z == 0) {
-            const uint4 w = *(const uint4 *)(codes + k_at(t, d0, Dp));
-            decode4<E4M3>(w.x, v);
-            decode4<E4M3>(w.y, v + 4);
-            decode4<E4M3>(w.z, v + 8);
-            decode4<E4M3>(w.w, v + 12);
-        } else {
-            const uint8_t *q = codes + v_at(t, d0, Dp);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                decode4<E4M3>(q[64 * j] | (uint32_t)q[64 * j + 16] << 8 | (uint32_t)q[64 * j + 32] << 16 | (uint32_t)q[64 * j + 48] << 24, v + 4 * j);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] *= s;
-    }
-    template <typename P, typename W>
-    __device__ void column(P &&p, W &&there, int d, float *v) const {
+    int first, here, full, shift, D, Dp, z;  // here: places of kept
+    bool late;  // some of the workgroup's tokens are in the old tail
+    struct Dims {
+        uint32_t w[4];
+        float s;
+    };
+    struct Column {
         uint32_t q[16];
         float s[16];
-        bool late = false;
+    };
+    __device__ void load(Dims &r, int p, int d0) const {
+        const int t = kept[p - first], tc = t < full ? t : 0;  // (token 0's place is there to be read)
+        if (z == 0) {
+            const uint4 w = *(const uint4 *)(codes + k_at(tc, d0, Dp));
+            r.w[0] = w.x, r.w[1] = w.y, r.w[2] = w.z, r.w[3] = w.w;
+        } else {
+            const uint8_t *q = codes + v_at(tc, d0, Dp);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int t = there(i) ? __builtin_amdgcn_readfirstlane(kept[p(i) - first]) : 0;
-            const int tc = t < full ? t : 0;  // (token 0's codes are there to be read)
-            late = late || t >= full;
-            q[i] = (codes + v_at(tc, 0, Dp))[(uint32_t)((d >> 4) * 1024 + (d & 15) * 16)];
-            s[i] = scales[tc / N];
+            for (int j = 0; j < 4; ++j)
+                r.w[j] = q[64 * j] | (uint32_t)q[64 * j + 16] << 8 | (uint32_t)q[64 * j + 32] << 16 | (uint32_t)q[64 * j + 48] << 24;
         }
+        r.s = scales[tc >> shift];
+    }
+    __device__ void values(const Dims &r, int p, int d0, float *v) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) decode4<E4M3>(q[4 * j] | q[4 * j + 1] << 8 | q[4 * j + 2] << 16 | q[4 * j + 3] << 24, v + 4 * j);
+        for (int j = 0; j < 4; ++j) decode4<E4M3>(r.w[j], v + 4 * j);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= s[i];
+        for (int e = 0; e < 16; ++e) v[e] *= r.s;
+        const int t = kept[p - first];
+        if (t >= full) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? tail[(int64_t)(t - full) * D + d0 + e] : 0.0f;
+        }
+    }
+    // (past the workgroup's tokens: its last)
+    __device__ int token(int t, int e) const { return __builtin_amdgcn_readfirstlane(kept[min(t + 16 * (e >> 2) + (e & 3) - first, here - 1)]); }
+    __device__ void load(Column &r, int t, int d) const {
+        const uint32_t at = (uint32_t)((d >> 4) * 1024 + (d & 15) * 16);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int u = token(t, e), uc = u < full ? u : 0;
+            r.q[e] = (codes + v_at(uc, 0, Dp))[at];
+            r.s[e] = scales[uc >> shift];
+        }
+    }
+    __device__ void values(const Column &r, int t, int d, float *v) const {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) decode4<E4M3>(r.q[4 * j] | r.q[4 * j + 1] << 8 | r.q[4 * j + 2] << 16 | r.q[4 * j + 3] << 24, v + 4 * j);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] *= r.s[e];
         if (late) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int t = there(i) ? __builtin_amdgcn_readfirstlane(kept[p(i) - first]) : 0;
-                if (t >= full) v[i] = tail[(int64_t)(t - full) * D + d];
+            for (int e = 0; e < 16; ++e) {
+                const int u = token(t, e);
+                if (u >= full) v[e] = d < D ? tail[(int64_t)(u - full) * D + d] : 0.0f;
             }
         }
     }
@@ -196,12 +209,12 @@ struct KeptSource {
 // NT tokens a workgroup, whole blocks of N.  `held` tokens were there, `total` are there afterwards; the workgroup
 // x of a (sequence, head) takes the x-th NT tokens from those of the block in progress on, t0 the first.
 template <bool E4M3, int DP, int NT, typename Source>
-__device__ inline void append_blocks(const Source &src, const Side &to, int N, int D, int z, int t0, int held, int total) {
+__device__ inline void append_blocks(const Source &src, const Side &to, int shift, int D, int z, int t0, int held, int total) {
     constexpr int ITEMS = NT * DP / 16 / kThreads, CH = DP / 16, BLOCKS = NT / 32;
     const int tid = threadIdx.x, lane = tid & 63;
     __shared__ uint32_t s_max[BLOCKS][kThreads / 64];
     // a block is written when it becomes full
-    auto fills = [&](int t) { return (t / N + 1) * N > held && (t / N + 1) * N <= total; };
+    auto fills = [&](int t) { return t >> shift >= held >> shift && t >> shift < total >> shift; };
     // item i of a thread.  K: dims 16 ch .. of token t, 16 lanes next to each other the 16 tokens of a tile, whose
     // chunk is contiguous in the codes.  V: the 16 tokens 16 kb + 4g + r of dim d, contiguous in the codes as well.
     auto k_token = [&](int i) { return t0 + i / (16 * CH) * 16 + (i & 15); };
@@ -214,35 +227,37 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int N, i
 #pragma unroll
     for (int b = 0; b < BLOCKS; ++b) amax[b] = 0;
     auto magnitude = [&](float v) { return __float_as_uint(v) & 0x7fffffffu; };
+    auto count = [&](int t, uint32_t most) {  // a block not to be written counts for nothing: its scale is not used
 #pragma unroll
-    for (int it = 0; it < ITEMS; ++it) {
-        const int i = tid + kThreads * it;
-        if (z == 0) {
-            const int t = k_token(i);
-            if (!fills(t)) continue;
-            src.dims(t, k_dim(i), x[it]);
+        for (int b = 0; b < BLOCKS; ++b) amax[b] = b == (t - t0) >> shift ? max(amax[b], most) : amax[b];
+    };
+    if (z == 0) {
+        typename Source::Dims raw[ITEMS];
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) src.load(raw[it], k_token(tid + kThreads * it), k_dim(tid + kThreads * it));
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int t = k_token(tid + kThreads * it);
+            src.values(raw[it], t, k_dim(tid + kThreads * it), x[it]);
             uint32_t most = 0;
 #pragma unroll
             for (int e = 0; e < 16; ++e) most = max(most, magnitude(x[it][e]));
+            count(t, most);
+        }
+    } else {
+        typename Source::Column raw[ITEMS];
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b) amax[b] = b == (t - t0) / N ? max(amax[b], most) : amax[b];
-        } else {
-            const int t = v_unit(i), d = i % DP;
-            if (!fills(t) && !fills(t + 32)) continue;
-            if (d < D) {
-                src.column([&](int e) { return t + 16 * (e >> 2) + (e & 3); }, [&](int e) { return fills(t + 16 * (e >> 2)); }, d, x[it]);
-            } else {
+        for (int it = 0; it < ITEMS; ++it) src.load(raw[it], v_unit(tid + kThreads * it), (tid + kThreads * it) % DP);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[it][e] = 0.0f;
-            }
+        for (int it = 0; it < ITEMS; ++it) {
+            const int t = v_unit(tid + kThreads * it);
+            src.values(raw[it], t, (tid + kThreads * it) % DP, x[it]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (!fills(t + 32 * h)) continue;
                 uint32_t most = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) most = max(most, magnitude(x[it][8 * h + e]));
-#pragma unroll
-                for (int b = 0; b < BLOCKS; ++b) amax[b] = b == (t + 32 * h - t0) / N ? max(amax[b], most) : amax[b];
+                count(t + 32 * h, most);
             }
         }
     }
@@ -260,13 +275,13 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int N, i
         const int e2 = bad ? 0 : scale_exponent(most, E4M3);
         // (a block with an infinity or NaN has no scale: all of it reads as NaN)
         inv[b] = bad ? NAN : __uint_as_float((uint32_t)(127 - e2) << 23);
-        if (tid == 0 && b * N < NT && fills(t0 + b * N))
-            to.scales[t0 / N + b] = bad ? NAN : __uint_as_float((uint32_t)(e2 + 127) << 23);
+        if (tid == 0 && b << shift < NT && fills(t0 + (b << shift)))
+            to.scales[(t0 >> shift) + b] = bad ? NAN : __uint_as_float((uint32_t)(e2 + 127) << 23);
     }
     auto inv_of = [&](int t) {
         float f = 0.0f;
 #pragma unroll
-        for (int b = 0; b < BLOCKS; ++b) f = b == (t - t0) / N ? inv[b] : f;
+        for (int b = 0; b < BLOCKS; ++b) f = b == (t - t0) >> shift ? inv[b] : f;
         return f;
     };
     auto encode = [&](const float *v, float f) {
@@ -288,7 +303,7 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int N, i
                 if (!fills(t + 32 * h)) {
                     // the unit's other block, of tokens to come: the attention reads it, with weights of 0, so it must not
                     // be e4m3 NaNs
-                    if (h == 1 && t + 32 >= total / N * N) o[1] = make_uint2(0u, 0u);
+                    if (h == 1 && t + 32 >= total >> shift << shift) o[1] = make_uint2(0u, 0u);
                     continue;
                 }
                 const float f = inv_of(t + 32 * h);
@@ -300,54 +315,98 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int N, i
 
 // The tokens after the last whole block, from token `from` of the cache on (those before are there): their values,
 // and the operands that the attention takes them as (the row divided by its own power of two, float16 hi + lo, in
-// the codes' order), DP / 16 lanes a row.  clear: zero operands behind them.
+// the codes' order).  First DP / 16 lanes a row, for its largest magnitude; K's operands are written there.  V's
+// lie with 16 tokens of a dim together: a few rows are written an element at a time, more (32 bytes a lane: a prompt's
+// tail of 17 rows took 14 us otherwise) from a second look at the tokens of the tail, the old ones among them.  clear:
+// zero operands behind them.
 template <int DP, typename Source>
-__device__ inline void append_tail(const Source &src, const Side &to, int N, int D, int z, int from, int total, bool clear) {
+__device__ inline void append_tail(const Source &src, const Side &to, int shift, int D, int z, int from, int total, bool clear) {
     constexpr int CH = DP / 16;
-    const int whole = total / N * N, room = max(N, kUnit), rows = clear ? room - (from - whole) : total - from;
-    for (int i = threadIdx.x; i < rows * CH; i += kThreads) {
-        const int p = from + i / CH, t = p - whole, d0 = i % CH * 16;
+    __shared__ float s_inv[kMaxBlock];  // a token's scale, inverted (0: not a finite row)
+    const int whole = total >> shift << shift, room = max(1 << shift, kUnit), rows = (clear ? whole + room : total) - from;
+    const bool columns = z == 1 && (rows > 4 || clear);
+    const int64_t plane = (int64_t)room * DP;
+    const int first = columns ? whole : from;
+    for (int i = threadIdx.x; i < (from + rows - first) * CH; i += kThreads) {
+        const int p = first + i / CH, t = p - whole, d0 = i % CH * 16;
+        const int pc = max(min(p, total - 1), first);  // (a row that is there; an empty cache's first has a place too)
         float v[16];
-        if (p < total) src.dims(p, d0, v);
-        float most = 0.0f;
+        typename Source::Dims raw;
+        src.load(raw, pc, d0);
+        src.values(raw, pc, d0, v);
+        uint32_t most = 0;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             v[e] = p < total ? v[e] : 0.0f;
-            most = fmaxf(most, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : INFINITY);
+            most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
         }
-        for (int m = CH / 2; m >= 1; m >>= 1) most = fmaxf(most, __shfl_xor(most, m, 64));
-        const bool bad = most == INFINITY;
-        const int e2 = bad || most == 0.0f ? -126 : min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
-        const float f = __uint_as_float((uint32_t)(127 - e2) << 23);
-        if (d0 == 0) to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
-        if (p < total) {
-            float *row = to.tail + (int64_t)t * D;
+        for (int m = CH / 2; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m, 64));
+        const bool bad = most >= 0x7f800000u;
+        const int e2 = bad || most == 0 ? -126 : min(max((int)(most >> 23) - 127, -126), 126);
+        const float f = bad ? 0.0f : __uint_as_float((uint32_t)(127 - e2) << 23);
+        if (d0 == 0) {
+            to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
+            s_inv[t] = f;
+        }
+        if (p >= from && p < total) {
+            float *row = to.tail + (int64_t)t * D + d0;
+            if (D % 16 == 0) {
+                if (d0 < D) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (d0 + e < D) row[d0 + e] = v[e];
+                    for (int e = 0; e < 4; ++e) ((float4 *)row)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (d0 + e < D) row[e] = v[e];
+            }
         }
-        _Float16 hi[16], lo[16];
+        if (columns) continue;
+        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+        half8 hi[2], lo[2];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float y = bad ? 0.0f : v[e] * f;
-            hi[e] = (_Float16)y;
-            lo[e] = (_Float16)(y - (float)hi[e]);
+            hi[e >> 3][e & 7] = (_Float16)y;
+            lo[e >> 3][e & 7] = (_Float16)(y - (float)hi[e >> 3][e & 7]);
         }
-        const int64_t plane = (int64_t)room * DP;
         if (z == 0) {
-            struct alignas(16) P {
-                _Float16 e[16];
-            };
-            *(P *)(to.ops + k_at(t, d0, DP)) = *(const P *)hi;
-            *(P *)(to.ops + plane + k_at(t, d0, DP)) = *(const P *)lo;
+            half8 *o = (half8 *)(to.ops + k_at(t, d0, DP));
+            o[0] = hi[0], o[1] = hi[1];
+            o = (half8 *)(to.ops + plane + k_at(t, d0, DP));
+            o[0] = lo[0], o[1] = lo[1];
         } else {
             _Float16 *o = to.ops + v_at(t, d0, DP);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                o[16 * e] = hi[e];
-                o[plane + 16 * e] = lo[e];
+                o[16 * e] = hi[e >> 3][e & 7];
+                o[plane + 16 * e] = lo[e >> 3][e & 7];
             }
         }
+    }
+    if (!columns) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < room / 16 * DP; i += kThreads) {
+        const int t = __builtin_amdgcn_readfirstlane(i / (4 * DP) * kUnit + 4 * (i / DP % 4)), d = i % DP;  // + 16 kb + r
+        if (!clear && whole + t >= total) continue;
+        float v[16];
+        typename Source::Column raw;
+        src.load(raw, whole + t, d);
+        src.values(raw, whole + t, d, v);
+        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+        half8 hi[2], lo[2];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int at = t + 16 * (e >> 2) + (e & 3);
+            const float f = whole + at < total ? s_inv[at] : 0.0f;
+            const float y = f == 0.0f ? 0.0f : v[e] * f;
+            hi[e >> 3][e & 7] = (_Float16)y;
+            lo[e >> 3][e & 7] = (_Float16)(y - (float)hi[e >> 3][e & 7]);
+        }
+        half8 *o = (half8 *)(to.ops + v_at(t, d, DP));
+        o[0] = hi[0], o[1] = hi[1];
+        o = (half8 *)(to.ops + plane + v_at(t, d, DP));
+        o[0] = lo[0], o[1] = lo[1];
     }
 }
 
@@ -355,10 +414,11 @@ template <int DP>
 __device__ inline Side slice(const Side &s, const AppendArgs &a, int64_t bg) {
     Side r;
     r.codes = s.codes + bg * a.units * kUnit * DP;
-    r.scales = s.scales + bg * (a.units * kUnit / a.N);
-    r.tail = s.tail + bg * a.N * a.D;
-    r.ops = s.ops + bg * 2 * max(a.N, kUnit) * DP;
-    r.op_scales = s.op_scales + bg * max(a.N, kUnit);
+    const int N = 1 << a.shift, room = max(N, kUnit);
+    r.scales = s.scales + bg * (a.units * kUnit >> a.shift);
+    r.tail = s.tail + bg * N * a.D;
+    r.ops = s.ops + bg * 2 * room * DP;
+    r.op_scales = s.op_scales + bg * room;
     return r;
 }
 
@@ -372,13 +432,14 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a
     const int t0 = (held / NT + (int)blockIdx.x) * NT;
     const Side to = slice<DP>(a.to[z], a, bg);
     const RowSource<T, VEC> src = {(const T *)a.src[z] + b * a.st[z][0] + g * a.st[z][1], a.st[z][2], a.st[z][3], to.tail,
-                                   held, held / a.N * a.N, a.D};
+                                   held, a.T, held >> a.shift << a.shift, a.D};
     // (a decode step that fills no block has none to look at)
-    if (held / a.N != total / a.N) append_blocks<E4M3, DP, NT>(src, to, a.N, a.D, z, t0, held, total);
-    // by the workgroup that has read the old tail
-    if (blockIdx.x != 0) return;
+    if (held >> a.shift != total >> a.shift) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, held, total);
+    // The new tail: by the workgroup of its tokens, or, where there is an old one, by the one that has read it.
+    const int from = max(held, total >> a.shift << a.shift), old = held & ((1 << a.shift) - 1);
+    if (from == total || (int)blockIdx.x != (old ? 0 : from / NT - held / NT)) return;
     __syncthreads();
-    append_tail<DP>(src, to, a.N, a.D, z, max(held, total / a.N * a.N), total, false);
+    append_tail<DP>(src, to, a.shift, a.D, z, from, total, false);
 }
 
 template <bool E4M3, int DP, int NT>
@@ -386,16 +447,21 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_evict_kernel(AppendArgs a)
     __shared__ int s_kept[NT];
     const int z = blockIdx.z;
     const int64_t bg = blockIdx.y, b = bg / a.Hkv;
-    const int total = min(a.len[b], a.keep), t0 = (int)blockIdx.x * NT;
+    const int total = min(a.len[b], a.keep), t0 = (int)blockIdx.x * NT, full = a.len[b] >> a.shift << a.shift;
     if (t0 >= total && (int)blockIdx.x > 0) return;  // (an empty sequence: its operands are cleared)
-    for (int i = threadIdx.x; i < min(NT, total - t0); i += kThreads) s_kept[i] = (int)a.kept[bg * a.keep + t0 + i];
-    __syncthreads();
+    bool late = false;
+    for (int i = threadIdx.x; i < NT; i += kThreads) {  // (places past the last token: token 0, not used)
+        const int t = t0 + i < total ? (int)a.kept[bg * a.keep + t0 + i] : 0;
+        s_kept[i] = t;
+        late = late || t >= full;
+    }
+    late = __syncthreads_or(late);
     const Side from = slice<DP>(a.from[z], a, bg), to = slice<DP>(a.to[z], a, bg);
-    const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, a.len[b] / a.N * a.N, a.N, a.D, DP, z};
-    append_blocks<E4M3, DP, NT>(src, to, a.N, a.D, z, t0, 0, total);
-    const int whole = total / a.N * a.N;
+    const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late};
+    append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
+    const int whole = total >> a.shift << a.shift;
     // the tail's tokens are among the last workgroup's, or there are none
-    if (total - t0 <= NT) append_tail<DP>(src, to, a.N, a.D, z, whole, total, true);
+    if (total - t0 <= NT) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
 }
 
 struct ReadArgs {
@@ -403,7 +469,7 @@ struct ReadArgs {
     const float *scales[2], *tail[2];
     void *out[2];            // dense (B, Hkv, rows, D)
     const int32_t *len;      // tokens held per sequence
-    int rows, Hkv, N, D, Dp;
+    int rows, Hkv, shift, D, Dp;
     int64_t units;
 };
 
@@ -414,12 +480,12 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
     // of a row, 8 dims each, read from different banks)
     constexpr int KP = 256 + 64, VP = 1024 + 16;
     __shared__ __attribute__((aligned(16))) uint8_t raw[kMaxDim / 16 * 4 * KP];
-    const int z = blockIdx.z, N = a.N, D = a.D, Dp = a.Dp, tid = threadIdx.x;
+    const int z = blockIdx.z, D = a.D, Dp = a.Dp, tid = threadIdx.x;
     const int64_t bg = blockIdx.y, b = bg / a.Hkv;
-    const int r0 = blockIdx.x * kUnit, held = a.len[b], full = held / N * N;
+    const int r0 = blockIdx.x * kUnit, held = a.len[b], full = held >> a.shift << a.shift;
     const uint8_t *codes = a.codes[z] + bg * a.units * kUnit * Dp;
-    const float *scales = a.scales[z] + bg * (a.units * kUnit / N);
-    const float *tail = a.tail[z] + bg * N * D;
+    const float *scales = a.scales[z] + bg * (a.units * kUnit >> a.shift);
+    const float *tail = a.tail[z] + (bg << a.shift) * D;
     TO *out = (TO *)a.out[z] + bg * (int64_t)a.rows * D;
     if (r0 < full) {
         for (int i = tid; i < kUnit * Dp / 16; i += kThreads)
@@ -450,7 +516,7 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
                 for (int j = 0; j < 2; ++j)
                     w[j] = p[64 * j] | (uint32_t)p[64 * j + 16] << 8 | (uint32_t)p[64 * j + 32] << 16 | (uint32_t)p[64 * j + 48] << 24;
             }
-            const float s = scales[t / N];
+            const float s = scales[t >> a.shift];
             decode4<E4M3>(w[0], v);
             decode4<E4M3>(w[1], v + 4);
 #pragma unroll
@@ -491,6 +557,8 @@ const void *evict_kernel(int Dp, int N) {
 #undef GT_E
 }
 
+int block_shift(int N) { return N == 32 ? 5 : N == 64 ? 6 : 7; }
+
 void fill_sides(Side *s, const gt_kv_blocks &c) {
     for (int z = 0; z < 2; ++z) s[z] = {(uint8_t *)c.codes[z], c.scales[z], c.tail[z], (_Float16 *)c.ops[z], c.op_scales[z]};
 }
@@ -527,7 +595,7 @@ hipError_t gt_launch_kv_blocks_append(const gt_kv_blocks &c, const void *const *
     a.pos_next = pos_next;
     a.T = (int)T;
     a.Hkv = (int)c.Hkv;
-    a.N = c.N;
+    a.shift = block_shift(c.N);
     a.D = (int)c.D;
     a.units = c.units;
     const void *kernel = src_dtype == GT_F32   ? append_kernel<float>(c.e4m3, vec, c.Dp, c.N)
@@ -545,7 +613,7 @@ hipError_t gt_launch_kv_blocks_evict(const gt_kv_blocks &from, const gt_kv_block
     a.kept = kept;
     a.keep = (int)keep;
     a.Hkv = (int)from.Hkv;
-    a.N = from.N;
+    a.shift = block_shift(from.N);
     a.D = (int)from.D;
     a.units = from.units;
     const int64_t nt = std::max(from.N, kUnit);
@@ -567,7 +635,7 @@ hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, i
     a.len = len;
     a.rows = (int)rows;
     a.Hkv = (int)c.Hkv;
-    a.N = c.N;
+    a.shift = block_shift(c.N);
     a.D = (int)c.D;
     a.Dp = c.Dp;
     a.units = c.units;
