@@ -67,7 +67,10 @@ class RoPEAxesFn(torch.autograd.Function):
         if grad_out is None:
             return (None,) * 9
         (pos,) = ctx.saved_tensors
-        gx = RoPEAxesFn.apply(grad_out, pos, *ctx.args, not ctx.inverse)
+        if torch.is_grad_enabled():  # (create_graph)
+            gx = RoPEAxesFn.apply(grad_out, pos, *ctx.args, not ctx.inverse)
+        else:
+            gx = _ops.rope_axes(grad_out, pos, *ctx.args, backward=not ctx.inverse)
         return (gx, None, None, None, None, None, None, None, None)
 
 

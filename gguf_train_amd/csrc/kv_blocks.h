@@ -46,6 +46,10 @@ GT_KVB_FN inline int64_t v_at(int64_t t, int d, int Dp) {
     return (t >> 6) * 64 * Dp + (d >> 4) * 1024 + ((kk >> 2) & 3) * 256 + (d & 15) * 16 + (kk >> 4) * 4 + (kk & 3);
 }
 
+// Whether token p waits in the tail of a cache that holds `held` tokens: row p - (held >> shift << shift), below
+// the tokens of a block (1 << shift).  A workgroup's span of 64 tokens may begin before that row 0.
+GT_KVB_FN inline bool in_tail(int p, int held, int shift) { return p < held && p >= held >> shift << shift; }
+
 // The scale's exponent for a block whose largest magnitude has the float32 bits `bits` (finite): the smallest
 // e >= -126 with amax <= top * 2^e, top 127 (int8) or 448 (e4m3).
 GT_KVB_FN inline int scale_exponent(uint32_t bits, bool e4m3) {

@@ -92,7 +92,7 @@ struct RowSource {
     const T *rows;
     int64_t sr, sd;
     const float *tail;
-    int held, count, blk0, D;  // blk0: the tail's first token
+    int held, count, shift, D;
     struct Dims {
         gtvec::Dims16<T> w;
         T y[VEC ? 1 : 16];
@@ -117,13 +117,14 @@ struct RowSource {
             else x = to_f(r.y[e]);
             v[e] = (VEC ? d0 : d0 + e) < D ? x : 0.0f;
         }
-        if (p < held) {  // waiting in the tail
+        if (in_tail(p, held, shift)) {
+            const float *waiting = tail + (int64_t)(p - (held >> shift << shift)) * D;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? tail[(int64_t)(p - blk0) * D + d0 + e] : 0.0f;
+            for (int e = 0; e < 16; ++e) v[e] = d0 + e < D ? waiting[d0 + e] : 0.0f;
         }
     }
     __device__ void load(Column &r, int t, int d) const {
-        const int at = min(d, D - 1) * (int)sd;
+        const int64_t at = min(d, D - 1) * sd;
 #pragma unroll
         for (int e = 0; e < 16; ++e) r.y[e] = row(t + 16 * (e >> 2) + (e & 3))[at];
     }
@@ -134,7 +135,7 @@ struct RowSource {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const int p = t + 16 * (e >> 2) + (e & 3);
-                if (p >= blk0 && p < held) v[e] = d < D ? tail[(int64_t)(p - blk0) * D + d] : 0.0f;
+                if (in_tail(p, held, shift)) v[e] = d < D ? tail[(int64_t)(p - (held >> shift << shift)) * D + d] : 0.0f;
             }
         }
     }
@@ -432,7 +433,7 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a
     const int t0 = (held / NT + (int)blockIdx.x) * NT;
     const Side to = slice<DP>(a.to[z], a, bg);
     const RowSource<T, VEC> src = {(const T *)a.src[z] + b * a.st[z][0] + g * a.st[z][1], a.st[z][2], a.st[z][3], to.tail,
-                                   held, a.T, held >> a.shift << a.shift, a.D};
+                                   held, a.T, a.shift, a.D};
     // (a decode step that fills no block has none to look at)
     if (held >> a.shift != total >> a.shift) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, held, total);
     // The new tail: by the workgroup of its tokens, or, where there is an old one, by the one that has read it.

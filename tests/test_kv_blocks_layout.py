@@ -42,6 +42,15 @@ int main(int argc, char **argv) {
                     for (int e = 0; e < 16; ++e)
                         if (v_at(64 * unit + 16 * (e / 4) + 4 * (lane / 16) + e % 4, 16 * i + lane % 16, Dp) != unit * 64 * Dp + 1024 * i + 16 * lane + e) return 4;
     }
+    // a tail row is read inside the tail, whatever span of tokens a workgroup looks at
+    for (int shift = 5; shift <= 7; ++shift)
+        for (int held = 0; held < 300; ++held)
+            for (int p = 0; p < 512; ++p) {
+                const int row = p - (held >> shift << shift);
+                const bool want = p < held && p / (1 << shift) == held / (1 << shift);
+                if (in_tail(p, held, shift) != want) return 6;
+                if (want && (row < 0 || row >= 1 << shift || row >= held % (1 << shift))) return 7;
+            }
     if (padded_dim(1) != 64 || padded_dim(64) != 64 || padded_dim(65) != 128 || padded_dim(129) != 256 || padded_dim(256) != 256) return 5;
     for (int i = 1; i < argc; ++i) {
         unsigned bits;
