@@ -5,11 +5,13 @@
 // with k_t = code x 2^a, v_t = code x 2^c, a and c a block's exponents.  HBM-bound: K and V are read once, a
 // byte a value.
 //
-// Rows: the G query heads of a kv head times the L tokens, r = head * L + token, are the columns of the matrix
-// instruction, 16 CT of them per workgroup; more take further workgroups over the same keys.  A workgroup owns
-// a span of 64-token units (a split of the sequence), its four wavefronts take them in turn, each with its own
-// running maximum and sum; they are joined once at the end, and the last split of a row group to finish joins
-// the splits (partials in uncached memory, as in decode_merge.h).
+// Rows: the G query heads of a kv head times the L tokens, r = head * L + token, are the 16 columns of the matrix
+// instruction; more than 16 take further workgroups over the same keys (two or four tiles of columns in a
+// workgroup, which decode the keys once for all, left one wavefront per SIMD and took longer: D128 32 rows of S1024
+// 19 against 16.5 us, 128 rows of S4096 42 against 35).  A workgroup owns a span of 64-token units (a split of the
+// sequence), its four wavefronts take them in turn, each with its own running maximum and sum; they are joined
+// once at the end, and the last split of a row group to finish joins the splits (partials in uncached memory, as
+// in decode_merge.h).
 //
 // Products on v_mfma_f32_16x16x32_f16, float32 sums.  Codes become float16 exactly: int8 (kept as code + 128) by placing
 // two bytes under exponent bytes (1024 + 128 + code) and subtracting 1152, e4m3 by the hardware's conversion.
@@ -50,6 +52,7 @@ using gtmfma::u32x4;
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
 constexpr int kWaves = 4;
+constexpr int kColumns = 16;  // rows of a workgroup
 
 struct AttnArgs {
     const void *q;
@@ -66,7 +69,6 @@ struct AttnArgs {
     int B, H, Hkv, L, D;
     int shift;  // log2 of the tokens of a block
     int64_t units;  // of a slice
-    int groups;     // row groups per kv head
     int nsplit, span;  // splits, units of each
     float *part_o, *part_ml;  // (rows, nsplit, Dp), (rows, nsplit, 2)
     int *counters;
@@ -128,20 +130,29 @@ __device__ inline void split8(const float *x, float inv, half8 &hi, half8 &lo) {
     }
 }
 
-// The B operands of one query row: lane (n, g) holds dims 16 (4i + g) .. +15 of its column's row, operand j the
-// eight from 8j on.  Returns the row's scale (the operands are the row divided by it).
+// A query row as lane (n, g) holds it: dims 16 (4i + g) .. +15 of its column's.  vec: aligned 16-byte pieces, D a
+// multiple of 16.
 template <typename QT, int NI>
-__device__ inline float load_query(const QT *row, int D, bool vec, int g, half8 (*hi)[2], half8 (*lo)[2]) {
-    constexpr bool F16 = __is_same(QT, _Float16);
-    float x[NI][16];
-    if (vec) {  // rows in aligned 16-byte pieces, D a multiple of 16
-        gtvec::Dims16<QT> raw[NI];
+struct QueryRow {
+    gtvec::Dims16<QT> raw[NI];
+    __device__ inline void load(const QT *row, int D, bool vec, int g) {
+        if (!vec) return;
 #pragma unroll
         for (int i = 0; i < NI; ++i) raw[i].load(row + (16 * (4 * i + g) < D ? 16 * (4 * i + g) : 0));
+    }
+};
+
+// Its B operands, operand j the eight dims from 8j on of the sixteen.  Returns the row's scale (the operands are the
+// row divided by it).
+template <typename QT, int NI>
+__device__ inline float query_operands(const QueryRow<QT, NI> &q, const QT *row, int D, bool vec, int g, half8 (*hi)[2], half8 (*lo)[2]) {
+    constexpr bool F16 = __is_same(QT, _Float16);
+    float x[NI][16];
+    if (vec) {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[i][e] = 16 * (4 * i + g) < D ? raw[i].get(e) : 0.0f;
+            for (int e = 0; e < 16; ++e) x[i][e] = 16 * (4 * i + g) < D ? q.raw[i].get(e) : 0.0f;
     } else {
 #pragma unroll
         for (int i = 0; i < NI; ++i)
@@ -172,10 +183,10 @@ __device__ inline float load_query(const QT *row, int D, bool vec, int g, half8 
 template <typename TO, int NI>
 __device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, float *lds) {
     constexpr int Dp = 64 * NI, PIECES = Dp / 4;
-    __shared__ float s_inv[64];
+    __shared__ float s_inv[kColumns];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ns = a.nsplit;  // ns <= 64
-    float mi[16], li[16];  // rows w, w + 4, ...: split `lane`
-    constexpr int RW = 64 / kWaves;
+    constexpr int RW = kColumns / kWaves;
+    float mi[RW], li[RW];  // rows w, w + 4, ...: split `lane`
 #pragma unroll
     for (int k = 0; k < RW; ++k) {
         const int r = w + kWaves * k;
@@ -231,112 +242,25 @@ GT_KVB_FN inline int64_t attn_lds_floats(int rows, int Dp, int nsplit) {
     return join > merge ? join : merge;
 }
 
-template <typename QT, int NI, int CT, bool E4M3>
-__global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
+template <typename QT, int NI, bool E4M3>
+__global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
     constexpr bool F32 = __is_same(QT, float);
-    constexpr int Dp = 64 * NI, COLS = 16 * CT, DT = 4 * NI;
+    constexpr int Dp = 64 * NI, DT = 4 * NI;
     constexpr int OP = Dp + 4;  // pitch of the rows to be joined
     extern __shared__ __attribute__((aligned(16))) float s_o[];  // [2][row]
-    __shared__ float s_m[kWaves][COLS], s_l[kWaves][COLS];
+    __shared__ float s_m[kWaves][kColumns], s_l[kWaves][kColumns];
     __shared__ int s_last;
 
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t x = blockIdx.x, bg = x / a.groups, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
-    const int rg = (int)(x - bg * a.groups), G = a.H / a.Hkv, rows = G * a.L;
-    const int r0 = rg * COLS, nr = min(COLS, rows - r0);
+    // row groups outermost: those of one slice land on the same XCD (workgroups are dealt round robin) when the slices
+    // are a multiple of 8, and share its L2
+    const int64_t x = blockIdx.x, slices = (int64_t)a.B * a.Hkv, bg = x % slices, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
+    const int rg = (int)(x / slices), G = a.H / a.Hkv, rows = G * a.L;
+    const int r0 = rg * kColumns, nr = min(kColumns, rows - r0);
     const int len = a.len[b], full = len >> a.shift << a.shift, tail = len - full;
 
-    // queries, and the first key that each column does not see
-    half8 qh[CT][NI][2], ql[CT][NI][2];
-    float f[CT];
-    int lim[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-        const int r = r0 + min(16 * ct + n, nr - 1), hh = r / a.L, l = r - hh * a.L;
-        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
-        f[ct] = load_query<QT, NI>(row, a.D, a.q_vec, g, qh[ct], ql[ct]) * a.scale * kLog2e;
-        lim[ct] = 16 * ct + n < nr ? (a.causal ? len - a.L + l + 1 : len) : 0;
-    }
-    const int lim_all = a.causal ? len - a.L + 1 : len;  // keys below it are seen by every row
-
-    float m[CT], mv[CT], lsum[CT];  // running max of s and of s + c, sum of 2^(s - m)
-    f32x4 acc[CT][DT];              // sum of 2^(s + c - mv) code
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-        m[ct] = mv[ct] = -INFINITY;
-        lsum[ct] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) acc[ct][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    // The softmax step over 64 keys from k0 on: c holds the column's products with the codes of keys 16 kb + 4g + i,
-    // ksc and vexp(kb, i) a key's scale and V exponent (PER_KEY: they differ within a kb); every key at or above
-    // `end` is not there.  Leaves p' as operands and rescales the sums.
-    auto softmax = [&](auto per_key, f32x4(&c)[CT][4], int k0, int end, auto &&ksc, auto &&vexp, half8(&ph)[CT][2], half8(&pl)[CT][2]) {
-        constexpr bool PER_KEY = decltype(per_key)::value;
-        const bool all = !PER_KEY && k0 + kUnit <= min(lim_all, end);
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) {
-            float cm = -INFINITY, cv = -INFINITY;
-            if (all) {
-                // every row sees every key: the scales are positive, so a kb's largest s is its largest product's
-#pragma unroll
-                for (int kb = 0; kb < 4; ++kb) {
-                    const f32x4 x = c[ct][kb];
-                    const float s = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * (f[ct] * ksc(kb, 0));
-                    cm = fmaxf(cm, s);
-                    cv = fmaxf(cv, s + vexp(kb, 0));
-                }
-            } else {
-#pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float s = c[ct][kb][i] * (f[ct] * ksc(kb, i));
-                        c[ct][kb][i] = k0 + 16 * kb + 4 * g + i < min(lim[ct], end) ? s : -INFINITY;
-                        cm = fmaxf(cm, c[ct][kb][i]);
-                        cv = fmaxf(cv, c[ct][kb][i] + vexp(kb, i));
-                    }
-            }
-            const float mn = fmaxf(m[ct], max_g(cm)), vn = fmaxf(mv[ct], max_g(cv));
-            const float ms = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m[ct] - mn);
-            const float beta = vn == -INFINITY ? 1.0f : fast_exp2(mv[ct] - vn);
-            const float shift = (vn == -INFINITY ? 0.0f : vn) - ms;
-            m[ct] = mn;
-            mv[ct] = vn;
-            float sum = 0.0f;
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-                const float fk = f[ct] * ksc(kb, 0);
-                float up = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = fast_exp2(all ? fmaf(c[ct][kb][i], fk, -ms) : c[ct][kb][i] - ms);
-                    sum += p;
-                    // 2^(c - r): where it passes 2^100, p is 0 or next to it; a NaN (a block that holds one) stays
-                    if (i == 0 || PER_KEY) {
-                        const float e = vexp(kb, i) - shift;
-                        up = fast_exp2(e > 100.0f ? 100.0f : e);
-                    }
-                    float pv = p * up;
-                    if (!all) pv = p == 0.0f ? 0.0f : pv;  // (a key that is not seen adds nothing, NaN or not)
-                    const int at = 4 * (kb & 1) + i;
-                    const _Float16 hi = (_Float16)pv;
-                    ph[ct][kb >> 1][at] = hi;
-                    if constexpr (F32) pl[ct][kb >> 1][at] = (_Float16)(pv - (float)hi);
-                }
-            }
-            lsum[ct] = fmaf(lsum[ct], alpha, sum_g(sum));
-            if (__builtin_amdgcn_ballot_w64(beta != 1.0f) != 0) {
-#pragma unroll
-                for (int t = 0; t < DT; ++t) acc[ct][t] *= beta;
-            }
-        }
-    };
-
-    // ---- whole blocks ----
+    // ---- whole blocks: the first unit's loads are on their way while the queries are made ready ----
     const int u0 = blockIdx.y * a.span, u1 = min(u0 + a.span, (full + kUnit - 1) / kUnit);
     const int64_t from = (bg * a.units + u0) * kUnit * Dp;
     // buffer loads: a uniform place, a lane's 16 bytes; past the last unit they return zeros and fetch nothing
@@ -359,7 +283,95 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
         for (int t = 0; t < DT; ++t)
             rv[t] = __builtin_amdgcn_raw_buffer_load_b128(vr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
     };
-    f32x4 c[CT][4];
+    if (u0 + w < u1) {
+        load_k(u0 + w);
+        load_v(u0 + w);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // the column's query, and the first key that it does not see
+    half8 qh[NI][2], ql[NI][2];
+    float f;
+    int lim;
+    {
+        const int r = r0 + min(n, nr - 1), hh = r / a.L, l = r - hh * a.L;
+        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
+        QueryRow<QT, NI> q;
+        q.load(row, a.D, a.q_vec, g);
+        f = query_operands<QT, NI>(q, row, a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e;
+        lim = n < nr ? (a.causal ? len - a.L + l + 1 : len) : 0;
+    }
+    const int lim_all = a.causal ? len - a.L + 1 : len;  // keys below it are seen by every row
+
+    float m = -INFINITY, mv = -INFINITY, lsum = 0.0f;  // running max of s and of s + c, sum of 2^(s - m)
+    f32x4 acc[DT];                                     // sum of 2^(s + c - mv) code
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // The softmax step over 64 keys from k0 on: c holds the column's products with the codes of keys 16 kb + 4g + i,
+    // ksc and vexp(kb, i) a key's scale and V exponent (PER_KEY: they differ within a kb); every key at or above
+    // `end` is not there.  Leaves p' as operands and rescales the sums.
+    f32x4 c[4];
+    half8 ph[2], pl[2];
+    auto softmax = [&](auto per_key, int k0, int end, auto &&ksc, auto &&vexp) {
+        constexpr bool PER_KEY = decltype(per_key)::value;
+        const bool all = !PER_KEY && k0 + kUnit <= min(lim_all, end);
+        float cm = -INFINITY, cv = -INFINITY;
+        if (all) {
+            // every row sees every key: the scales are positive, so a kb's largest s is its largest product's
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) {
+                const float s = fmaxf(fmaxf(c[kb][0], c[kb][1]), fmaxf(c[kb][2], c[kb][3])) * (f * ksc(kb, 0));
+                cm = fmaxf(cm, s);
+                cv = fmaxf(cv, s + vexp(kb, 0));
+            }
+        } else {
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float s = c[kb][i] * (f * ksc(kb, i));
+                    c[kb][i] = k0 + 16 * kb + 4 * g + i < min(lim, end) ? s : -INFINITY;
+                    cm = fmaxf(cm, c[kb][i]);
+                    cv = fmaxf(cv, c[kb][i] + vexp(kb, i));
+                }
+        }
+        const float mn = fmaxf(m, max_g(cm)), vn = fmaxf(mv, max_g(cv));
+        const float ms = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = mn == -INFINITY ? 1.0f : fast_exp2(m - mn);
+        const float beta = vn == -INFINITY ? 1.0f : fast_exp2(mv - vn);
+        const float shift = (vn == -INFINITY ? 0.0f : vn) - ms;
+        m = mn;
+        mv = vn;
+        float sum = 0.0f;
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const float fk = f * ksc(kb, 0);
+            float up = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = fast_exp2(all ? fmaf(c[kb][i], fk, -ms) : c[kb][i] - ms);
+                sum += p;
+                // 2^(c - r): where it passes 2^100, p is 0 or next to it; a NaN (a block that holds one) stays
+                if (i == 0 || PER_KEY) {
+                    const float e = vexp(kb, i) - shift;
+                    up = fast_exp2(e > 100.0f ? 100.0f : e);
+                }
+                float pv = p * up;
+                if (!all) pv = p == 0.0f ? 0.0f : pv;  // (a key that is not seen adds nothing, NaN or not)
+                const int at = 4 * (kb & 1) + i;
+                const _Float16 hi = (_Float16)pv;
+                ph[kb >> 1][at] = hi;
+                if constexpr (F32) pl[kb >> 1][at] = (_Float16)(pv - (float)hi);
+            }
+        }
+        lsum = fmaf(lsum, alpha, sum_g(sum));
+        if (__builtin_amdgcn_ballot_w64(beta != 1.0f) != 0) {
+#pragma unroll
+            for (int t = 0; t < DT; ++t) acc[t] *= beta;
+        }
+    };
+
     float sk[4], ev[4];
     auto scores = [&]() {
 #pragma unroll
@@ -367,24 +379,16 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
             sk[kb] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(rs), kb));
             ev[kb] = exponent_bits(__builtin_amdgcn_readlane(__float_as_uint(rs), 4 + kb));
             __builtin_amdgcn_sched_barrier(0);  // (one tile's operands at a time: registers)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            c[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const half8 ka = decode8<E4M3>(rk[kb * NI + i][2 * j], rk[kb * NI + i][2 * j + 1]);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        if constexpr (F32) c[ct][kb] = mma(ka, ql[ct][i][j], c[ct][kb]);
-                        c[ct][kb] = mma(ka, qh[ct][i][j], c[ct][kb]);
-                    }
+                    if constexpr (F32) c[kb] = mma(ka, ql[i][j], c[kb]);
+                    c[kb] = mma(ka, qh[i][j], c[kb]);
                 }
         }
-    };
-    half8 ph[CT][2], pl[CT][2];
-    auto weigh = [&](int u) {
-        softmax(std::false_type{}, c, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; }, ph, pl);
     };
     auto values = [&]() {
 #pragma unroll
@@ -393,23 +397,16 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const half8 va = decode8<E4M3>(rv[t][2 * j], rv[t][2 * j + 1]);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    if constexpr (F32) acc[ct][t] = mma(va, pl[ct][j], acc[ct][t]);
-                    acc[ct][t] = mma(va, ph[ct][j], acc[ct][t]);
-                }
+                if constexpr (F32) acc[t] = mma(va, pl[j], acc[t]);
+                acc[t] = mma(va, ph[j], acc[t]);
             }
         }
     };
     // the next unit's K is on its way during the softmax and P.V, its V during the next scores
-    if (u0 + w < u1) {
-        load_k(u0 + w);
-        load_v(u0 + w);
-    }
     for (int u = u0 + w; u < u1; u += kWaves) {
         scores();
         load_k(u + kWaves);
-        weigh(u);
+        softmax(std::false_type{}, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; });
         values();
         load_v(u + kWaves);
     }
@@ -430,9 +427,8 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
             const f32x4 vs = *(const f32x4 *)(a.vts + bg * room + t0 + 16 * kb + 4 * g);
 #pragma unroll
             for (int i = 0; i < 4; ++i) vex[kb][i] = exponent_bits(__float_as_uint(vs[i]));
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) c[ct][kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            __builtin_amdgcn_sched_barrier(0);  // (one tile's operands at a time: registers)
+            c[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (kb == 2) __builtin_amdgcn_sched_barrier(0);  // (two tiles' operands at a time: registers)
             if (t0 + 16 * kb >= tail) continue;
 #pragma unroll
             for (int i = 0; i < NI; ++i)
@@ -440,57 +436,44 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
                 for (int j = 0; j < 2; ++j) {
                     const half8 hi = *(const half8 *)(kt + kb * 16 * Dp + 1024 * i + 8 * j);
                     const half8 lo = *(const half8 *)(kt + lo_at + kb * 16 * Dp + 1024 * i + 8 * j);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ++ct) {
-                        if constexpr (F32) c[ct][kb] = mma(hi, ql[ct][i][j], c[ct][kb]);
-                        c[ct][kb] = mma(lo, qh[ct][i][j], c[ct][kb]);
-                        c[ct][kb] = mma(hi, qh[ct][i][j], c[ct][kb]);
-                    }
+                    if constexpr (F32) c[kb] = mma(hi, ql[i][j], c[kb]);
+                    c[kb] = mma(lo, qh[i][j], c[kb]);
+                    c[kb] = mma(hi, qh[i][j], c[kb]);
                 }
         }
-        softmax(std::true_type{}, c, full + t0, len, [&](int kb, int i) { return ksc[kb][i]; }, [&](int kb, int i) { return vex[kb][i]; }, ph, pl);
+        softmax(std::true_type{}, full + t0, len, [&](int kb, int i) { return ksc[kb][i]; }, [&](int kb, int i) { return vex[kb][i]; });
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                if (j == 0) __builtin_amdgcn_sched_barrier(0);
+                if (j == 0 && t % 4 == 0) __builtin_amdgcn_sched_barrier(0);
                 if (t0 + 32 * j >= tail) continue;  // (operand j: tokens 32 j .. +31)
                 const half8 hi = *(const half8 *)(vt + 1024 * t + 8 * j), lo = *(const half8 *)(vt + lo_at + 1024 * t + 8 * j);
-#pragma unroll
-                for (int ct = 0; ct < CT; ++ct) {
-                    if constexpr (F32) acc[ct][t] = mma(hi, pl[ct][j], acc[ct][t]);
-                    acc[ct][t] = mma(lo, ph[ct][j], acc[ct][t]);
-                    acc[ct][t] = mma(hi, ph[ct][j], acc[ct][t]);
-                }
+                if constexpr (F32) acc[t] = mma(hi, pl[j], acc[t]);
+                acc[t] = mma(lo, ph[j], acc[t]);
+                acc[t] = mma(hi, ph[j], acc[t]);
             }
     }
 
     // ---- join the wavefronts, in order ----
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct)
-        if (g == 0) {
-            s_m[w][16 * ct + n] = m[ct];
-            s_l[w][16 * ct + n] = lsum[ct];
-        }
+    if (g == 0) {
+        s_m[w][n] = m;
+        s_l[w][n] = lsum;
+    }
     __syncthreads();
     // waves 2 and 3 leave theirs, waves 0 and 1 add their own
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
-        if ((w >> 1) == half) {
+        if ((w >> 1) == half && n < nr) {
+            const float M = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+            const float to = mv == -INFINITY ? 0.0f : fast_exp2(mv - (M == -INFINITY ? 0.0f : M));
+            const bool bad = lsum != lsum;
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) {
-                const int col = 16 * ct + n;
-                if (col >= nr) continue;
-                const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
-                const float to = mv[ct] == -INFINITY ? 0.0f : fast_exp2(mv[ct] - (M == -INFINITY ? 0.0f : M));
-                const bool bad = lsum[ct] != lsum[ct];
-#pragma unroll
-                for (int t = 0; t < DT; ++t) {
-                    f32x4 y = acc[ct][t] * to;
-                    if (bad) y = f32x4{NAN, NAN, NAN, NAN};
-                    f32x4 *o = (f32x4 *)&s_o[((w & 1) * nr + col) * OP + 16 * t + 4 * g];
-                    *o = half == 0 ? *o + y : y;
-                }
+            for (int t = 0; t < DT; ++t) {
+                f32x4 y = acc[t] * to;
+                if (bad) y = f32x4{NAN, NAN, NAN, NAN};
+                f32x4 *o = (f32x4 *)&s_o[((w & 1) * nr + n) * OP + 16 * t + 4 * g];
+                *o = half == 0 ? *o + y : y;
             }
         }
         __syncthreads();
@@ -531,25 +514,16 @@ __global__ __launch_bounds__(64 * kWaves, CT == 1 && NI <= 2 ? 2 : 1) void attn_
     if (threadIdx.x == 0) __hip_atomic_store(&a.counters[x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The kernel for head sizes padded to Dp and up to 16 ct rows a workgroup; null when there is none (ct Dp / 64
-// <= 4: past it the sums of P.V and the queries do not stay in registers).
+// The kernel for head sizes padded to Dp.
 template <typename QT>
-inline const void *attn_kernel(int Dp, int ct, bool e4m3) {
-#define GT_K(NI, CT) (e4m3 ? (const void *)attn_kv_blocks_kernel<QT, NI, CT, true> : (const void *)attn_kv_blocks_kernel<QT, NI, CT, false>)
-    switch (Dp / 64 * 10 + ct) {
-        case 11: return GT_K(1, 1);
-        case 12: return GT_K(1, 2);
-        case 14: return GT_K(1, 4);
-        case 21: return GT_K(2, 1);
-        case 22: return GT_K(2, 2);
-        case 41: return GT_K(4, 1);
-        default: return nullptr;
-    }
+inline const void *attn_kernel(int Dp, bool e4m3) {
+#define GT_K(NI) (e4m3 ? (const void *)attn_kv_blocks_kernel<QT, NI, true> : (const void *)attn_kv_blocks_kernel<QT, NI, false>)
+    return Dp == 64 ? GT_K(1) : Dp == 128 ? GT_K(2) : GT_K(4);
 #undef GT_K
 }
 
-const void *attn_kernel_f16(int Dp, int ct, bool e4m3);
-const void *attn_kernel_bf16(int Dp, int ct, bool e4m3);
-const void *attn_kernel_f32(int Dp, int ct, bool e4m3);
+const void *attn_kernel_f16(int Dp, bool e4m3);
+const void *attn_kernel_bf16(int Dp, bool e4m3);
+const void *attn_kernel_f32(int Dp, bool e4m3);
 
 }  // namespace gtkvb

@@ -9,11 +9,11 @@ namespace {
 
 using namespace gtkvb;
 
-const void *kernel_of(int q_dtype, int Dp, int ct, bool e4m3) {
+const void *kernel_of(int q_dtype, int Dp, bool e4m3) {
     switch (q_dtype) {
-        case GT_F16: return attn_kernel_f16(Dp, ct, e4m3);
-        case GT_BF16: return attn_kernel_bf16(Dp, ct, e4m3);
-        case GT_F32: return attn_kernel_f32(Dp, ct, e4m3);
+        case GT_F16: return attn_kernel_f16(Dp, e4m3);
+        case GT_BF16: return attn_kernel_bf16(Dp, e4m3);
+        case GT_F32: return attn_kernel_f32(Dp, e4m3);
         default: return nullptr;
     }
 }
@@ -69,14 +69,10 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
     a.D = (int)c.D;
     a.shift = c.N == 32 ? 5 : c.N == 64 ? 6 : 7;
     a.units = c.units;
-    // columns of a workgroup: the fewest that hold the rows, as many as the head size allows
-    const int64_t rows = r.H / c.Hkv * r.L;
-    int ct = 1;
-    while (16 * ct < rows && 2 * ct * (c.Dp / 64) <= 4) ct *= 2;
-    a.groups = (int)((rows + 16 * ct - 1) / (16 * ct));
-    const void *kernel = kernel_of(r.q_dtype, c.Dp, ct, c.e4m3);
+    const int64_t rows = r.H / c.Hkv * r.L, groups = (rows + kColumns - 1) / kColumns;
+    const void *kernel = kernel_of(r.q_dtype, c.Dp, c.e4m3);
     if (!kernel) return hipErrorInvalidValue;
-    const int64_t grid = c.B * c.Hkv * a.groups;
+    const int64_t grid = c.B * c.Hkv * groups;
     if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
     // splits: a workgroup's four wavefronts take a unit each per step
     const int64_t units = (r.max_len / c.N * c.N + kUnit - 1) / kUnit, steps = std::max<int64_t>(1, (units + kWaves - 1) / kWaves);
@@ -98,9 +94,9 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
     a.nsplit = n;
     a.span = (int)(per * kWaves);
     note = std::string("decode ") + (c.e4m3 ? "e4m3" : "int8") + " blocks of " + std::to_string(c.N) + " D=" + std::to_string(c.D) +
-           " rows=" + std::to_string(rows) + " columns=" + std::to_string(16 * ct) + " splits=" + std::to_string(n) +
+           " rows=" + std::to_string(rows) + " splits=" + std::to_string(n) +
            " units=" + std::to_string(grid);
     void *args[] = {(void *)&a};
-    const size_t lds = (size_t)attn_lds_floats((int)std::min<int64_t>(rows, 16 * ct), c.Dp, n) * sizeof(float);
+    const size_t lds = (size_t)attn_lds_floats((int)std::min<int64_t>(rows, kColumns), c.Dp, n) * sizeof(float);
     return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3(64 * kWaves), args, lds, s);
 }

@@ -1,4 +1,4 @@
 // attn_kv_blocks.h for bfloat16 queries.
 #include "attn_kv_blocks.h"
 
-const void *gtkvb::attn_kernel_bf16(int Dp, int ct, bool e4m3) { return attn_kernel<__bf16>(Dp, ct, e4m3); }
+const void *gtkvb::attn_kernel_bf16(int Dp, bool e4m3) { return attn_kernel<__bf16>(Dp, e4m3); }

@@ -26,9 +26,9 @@ __device__ inline float to_f(T x) {
 }
 // A finite value stays finite: amax rounds up to a code's value, past float16's largest for amax near it.
 template <typename T>
-__device__ inline T from_f(float x) {
-    if constexpr (__is_same(T, _Float16)) x = fabsf(x) < INFINITY && fabsf(x) > 65504.0f ? copysignf(65504.0f, x) : x;
-    return (T)x;
+__device__ inline float finite(float x) {
+    if constexpr (__is_same(T, _Float16)) return fabsf(x) < INFINITY && fabsf(x) > 65504.0f ? copysignf(65504.0f, x) : x;
+    return x;
 }
 
 // Four values already divided by the scale, as codes (round to nearest even).
@@ -141,14 +141,22 @@ struct RowSource {
     }
 };
 
-// Tokens of another block cache (z 0 keys, 1 values): token `first` + i of the new cache is kept[i], in LDS.
-template <bool E4M3>
+// The V codes of a few units in LDS, 16 dims at a pitch that puts a wavefront's bytes, 16 apart, into different banks
+// two by two.
+constexpr int kStagedUnits = 3, kStagedPitch = 1024 + 8;
+
+// Tokens of another block cache (z 0 keys, 1 values): token `first` + i of the new cache is kept[i], in LDS.  A
+// token's V codes are 16 bytes apart, so that a wavefront's 64 take 16 lines of which the others hold other tokens':
+// STAGED, the units of all the workgroup's tokens are in LDS, from unit `unit0` on (columns only).
+template <bool E4M3, bool STAGED>
 struct KeptSource {
     const uint8_t *codes;
     const float *scales, *tail;
     const int *kept;
     int first, here, full, shift, D, Dp, z;  // here: places of kept
     bool late;  // some of the workgroup's tokens are in the old tail
+    const uint8_t *staged;
+    int unit0;
     struct Dims {
         uint32_t w[4];
         float s;
@@ -184,12 +192,19 @@ struct KeptSource {
     // (past the workgroup's tokens: its last)
     __device__ int token(int t, int e) const { return __builtin_amdgcn_readfirstlane(kept[min(t + 16 * (e >> 2) + (e & 3) - first, here - 1)]); }
     __device__ void load(Column &r, int t, int d) const {
-        const uint32_t at = (uint32_t)((d >> 4) * 1024 + (d & 15) * 16);
+        const uint32_t at = (uint32_t)((d >> 4) * (STAGED ? kStagedPitch : 1024) + (d & 15) * 16);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int u = token(t, e), uc = u < full ? u : 0;
-            r.q[e] = (codes + v_at(uc, 0, Dp))[at];
-            r.s[e] = scales[uc >> shift];
+            const int u = token(t, e);
+            if constexpr (STAGED) {
+                const int uc = u < full && u >= unit0 * kUnit ? u : unit0 * kUnit;
+                r.q[e] = staged[((uc >> 6) - unit0) * (Dp / 16) * kStagedPitch + (int)v_at(uc & 63, 0, Dp) + (int)at];
+                r.s[e] = scales[uc >> shift];
+            } else {
+                const int uc = u < full ? u : 0;
+                r.q[e] = (codes + v_at(uc, 0, Dp))[at];
+                r.s[e] = scales[uc >> shift];
+            }
         }
     }
     __device__ void values(const Column &r, int t, int d, float *v) const {
@@ -458,11 +473,27 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_evict_kernel(AppendArgs a)
     }
     late = __syncthreads_or(late);
     const Side from = slice<DP>(a.from[z], a, bg), to = slice<DP>(a.to[z], a, bg);
-    const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late};
-    append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
     const int whole = total >> a.shift << a.shift;
-    // the tail's tokens are among the last workgroup's, or there are none
-    if (total - t0 <= NT) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
+    const bool last = total - t0 <= NT;  // the tail's tokens are among the last workgroup's, or there are none
+    auto write = [&](const auto &src) {
+        append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
+        if (last) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
+    };
+    // the tokens are in order: their units
+    const int unit0 = s_kept[0] >> 6, units = (min(s_kept[max(min(NT, total - t0), 1) - 1], full - 1) >> 6) - unit0 + 1;
+    if (z == 1 && !last && units >= 1 && units <= kStagedUnits) {
+        __shared__ __attribute__((aligned(16))) uint8_t s_codes[kStagedUnits * (DP / 16) * kStagedPitch];
+        for (int i = threadIdx.x; i < units * 4 * DP; i += kThreads) {
+            const uint4 w = *(const uint4 *)(from.codes + (int64_t)unit0 * kUnit * DP + 16 * i);
+            uint2 *o = (uint2 *)(s_codes + i / 64 * kStagedPitch + i % 64 * 16);
+            o[0] = make_uint2(w.x, w.y);
+            o[1] = make_uint2(w.z, w.w);
+        }
+        __syncthreads();
+        write(KeptSource<E4M3, true>{from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late, s_codes, unit0});
+    } else {
+        write(KeptSource<E4M3, false>{from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late, nullptr, 0});
+    }
 }
 
 struct ReadArgs {
@@ -504,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
             for (int e = 0; e < 8; ++e) v[e] = 0.0f;
         } else if (t >= full) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = d0 + e < D ? tail[(int64_t)(t - full) * D + d0 + e] : 0.0f;
+            for (int e = 0; e < 8; ++e) v[e] = d0 + e < D ? finite<TO>(tail[(int64_t)(t - full) * D + d0 + e]) : 0.0f;
         } else {
             uint32_t w[2];
             if (z == 0) {
@@ -518,10 +549,20 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
                     w[j] = p[64 * j] | (uint32_t)p[64 * j + 16] << 8 | (uint32_t)p[64 * j + 32] << 16 | (uint32_t)p[64 * j + 48] << 24;
             }
             const float s = scales[t >> a.shift];
-            decode4<E4M3>(w[0], v);
-            decode4<E4M3>(w[1], v + 4);
+            if (!E4M3 && s < 128.0f) {
+                // (byte - 128) s in one step: the product and the difference are exact
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= s;
+                for (int e = 0; e < 8; ++e) v[e] = fmaf((float)(w[e >> 2] >> (8 * (e & 3)) & 0xffu), s, -128.0f * s);
+            } else {
+                decode4<E4M3>(w[0], v);
+                decode4<E4M3>(w[1], v + 4);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= s;
+                if (s >= 128.0f) {  // (448 s passes float16's largest)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[e] = finite<TO>(v[e]);
+                }
+            }
         }
         TO *o = out + (int64_t)(r0 + r) * D + d0;
         if (D % 8 == 0) {
@@ -529,12 +570,12 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_read_kernel(ReadArgs a) {
                 TO e[8];
             } p;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p.e[e] = from_f<TO>(v[e]);
+            for (int e = 0; e < 8; ++e) p.e[e] = (TO)v[e];
             *(P *)o = p;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (d0 + e < D) o[e] = from_f<TO>(v[e]);
+                if (d0 + e < D) o[e] = (TO)v[e];
         }
     }
 }
