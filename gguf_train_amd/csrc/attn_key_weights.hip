@@ -194,26 +194,16 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
         for (int i = 0; i < 4; ++i) sum[kb][i] = 0.0f;
     const int G = a.H / a.Hkv, rows = G * a.L;
     const int c0 = blockIdx.z * a.span, c1 = min(c0 + a.span, a.col_tiles);
-    // column ct's row of this lane; the next column's is on its way during this one's products
-    auto row_of = [&](int ct) {
-        const int r = min(16 * ct + n, rows - 1), hh = r / a.L, l = r - hh * a.L;
-        return (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
-    };
-    const float *lse = a.lse + (b * a.H + kvh * G) * a.L;
-    QueryRow<QT, NI> next;
-    next.load(row_of(c0), a.D, a.q_vec, g);
-    float next_lse = lse[min(16 * c0 + n, rows - 1)];
     for (int ct = c0; ct < c1; ++ct) {
-        const int rr = 16 * ct + n, l = min(rr, rows - 1) % a.L;
+        const int rr = 16 * ct + n, r = min(rr, rows - 1), hh = r / a.L, l = r - hh * a.L;
         const int lim = rr < rows ? (a.causal ? len - a.L + l + 1 : len) : 0;
-        const QueryRow<QT, NI> q = next;
-        const float ls = next_lse * kLog2e;
-        const int after = min(ct + 1, c1 - 1);
-        next.load(row_of(after), a.D, a.q_vec, g);
-        next_lse = lse[min(16 * after + n, rows - 1)];
         if (__builtin_amdgcn_ballot_w64(lim > k0) == 0) continue;
         half8 qh[NI][2], ql[NI][2];
-        const float f = query_operands<QT, NI>(q, row_of(ct), a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e;
+        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
+        QueryRow<QT, NI> q;
+        q.load(row, a.D, a.q_vec, g);
+        const float ls = a.lse[(b * a.H + kvh * G) * a.L + r] * kLog2e;
+        const float f = query_operands<QT, NI>(q, row, a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e;
 #pragma unroll
         for (int kb = 0; kb < TW; ++kb) {
             f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -229,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
                 }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = fast_exp2(c[i] * (f * ksc[kb][i]) - ls);
+                const float p = fast_exp2(fmaf(c[i], f * ksc[kb][i], -ls));
                 sum[kb][i] += k0 + 16 * kb + 4 * g + i < lim ? p : 0.0f;
             }
         }

@@ -147,6 +147,18 @@ struct QueryRow {
 template <typename QT, int NI>
 __device__ inline float query_operands(const QueryRow<QT, NI> &q, const QT *row, int D, bool vec, int g, half8 (*hi)[2], half8 (*lo)[2]) {
     constexpr bool F16 = __is_same(QT, _Float16);
+    if constexpr (F16) {
+        if (vec) {  // its own operand
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const u32x4 w = q.raw[i].w[j];
+                    hi[i][j] = __builtin_bit_cast(half8, 16 * (4 * i + g) < D ? w : u32x4{0u, 0u, 0u, 0u});
+                }
+            return 1.0f;
+        }
+    }
     float x[NI][16];
     if (vec) {
 #pragma unroll

@@ -334,28 +334,28 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int shif
 // the codes' order).  First DP / 16 lanes a row, for its largest magnitude; K's operands are written there.  V's
 // lie with 16 tokens of a dim together: a few rows are written an element at a time, more (32 bytes a lane: a prompt's
 // tail of 17 rows took 14 us otherwise) from a second look at the tokens of the tail, the old ones among them.  clear:
-// zero operands behind them.
+// the operands of tokens to come become zeros.
 template <int DP, typename Source>
 __device__ inline void append_tail(const Source &src, const Side &to, int shift, int D, int z, int from, int total, bool clear) {
     constexpr int CH = DP / 16;
     __shared__ float s_inv[kMaxBlock];  // a token's scale, inverted (0: not a finite row)
-    const int whole = total >> shift << shift, room = max(1 << shift, kUnit), rows = (clear ? whole + room : total) - from;
-    const bool columns = z == 1 && (rows > 4 || clear);
+    const int whole = total >> shift << shift, room = max(1 << shift, kUnit), rows = total - from;
+    const bool columns = z == 1 && rows > 4;
     const int64_t plane = (int64_t)room * DP;
     const int first = columns ? whole : from;
-    for (int i = threadIdx.x; i < (from + rows - first) * CH; i += kThreads) {
+    if (clear) {
+        for (int i = threadIdx.x; i < (int)(plane / 4); i += kThreads) ((uint4 *)to.ops)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < (total - first) * CH; i += kThreads) {
         const int p = first + i / CH, t = p - whole, d0 = i % CH * 16;
-        const int pc = max(min(p, total - 1), first);  // (a row that is there; an empty cache's first has a place too)
         float v[16];
         typename Source::Dims raw;
-        src.load(raw, pc, d0);
-        src.values(raw, pc, d0, v);
+        src.load(raw, p, d0);
+        src.values(raw, p, d0, v);
         uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            v[e] = p < total ? v[e] : 0.0f;
-            most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
-        }
+        for (int e = 0; e < 16; ++e) most = max(most, __float_as_uint(v[e]) & 0x7fffffffu);
         for (int m = CH / 2; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m, 64));
         const bool bad = most >= 0x7f800000u;
         const int e2 = bad || most == 0 ? -126 : min(max((int)(most >> 23) - 127, -126), 126);
@@ -364,7 +364,7 @@ __device__ inline void append_tail(const Source &src, const Side &to, int shift,
             to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
             s_inv[t] = f;
         }
-        if (p >= from && p < total) {
+        if (p >= from) {
             float *row = to.tail + (int64_t)t * D + d0;
             if (D % 16 == 0) {
                 if (d0 < D) {
@@ -404,7 +404,7 @@ __device__ inline void append_tail(const Source &src, const Side &to, int shift,
     __syncthreads();
     for (int i = threadIdx.x; i < room / 16 * DP; i += kThreads) {
         const int t = __builtin_amdgcn_readfirstlane(i / (4 * DP) * kUnit + 4 * (i / DP % 4)), d = i % DP;  // + 16 kb + r
-        if (!clear && whole + t >= total) continue;
+        if (whole + t >= total) continue;
         float v[16];
         typename Source::Column raw;
         src.load(raw, whole + t, d);
