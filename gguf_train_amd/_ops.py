@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -180,10 +181,14 @@ def rope(x, pos, n_dims: int, mode: int = 0, n_ctx_orig: int = 0, freq_base: flo
     return adopt(ptr, "rope")
 
 
+@functools.lru_cache(maxsize=64)
+def _section_array(sections: tuple):
+    return len(sections), (ctypes.c_int * max(len(sections), 1))(*sections)
+
+
 def section_list(sections):
     """(count, C array) of the pairs per axis; the entry points check the numbers."""
-    vals = [int(n) for n in sections]
-    return len(vals), (ctypes.c_int * max(len(vals), 1))(*vals)
+    return _section_array(tuple(map(int, sections)))
 
 
 def rope_axes(x, pos, sections, n_dims: int, mode: int = 2, interleaved: bool = False, freq_base: float = 10000.0,

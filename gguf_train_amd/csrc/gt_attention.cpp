@@ -2107,7 +2107,7 @@ int kv_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weig
     }
     ok = ok && gt_hip_check(gt_launch_kv_select((const float *)gt_data(w), w->strides, len, (int32_t *)gt_data(c->len_next),
                                                 c->evicted ? (int32_t *)gt_data(c->evicted) : nullptr, (int64_t *)gt_data(kept), B, Hkv,
-                                                keep, recent, gt_stream()),
+                                                max_len, keep, recent, gt_stream()),
                             "kv cache select kernel");
     if (cut) {
         // a block cache's kept tokens are quantized again in their new blocks (exactly where the scale stays or

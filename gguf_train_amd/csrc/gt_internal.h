@@ -225,7 +225,7 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
 // largest weights w (element strides), in order; a sequence of at most `keep` tokens keeps them (-1 behind).
 // next[b]: the length afterwards; evicted[b] grows by what is lost (null: no sequence is longer than keep).
 hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int32_t *next, int32_t *evicted, int64_t *kept,
-                               int64_t B, int64_t Hkv, int64_t keep, int64_t recent, hipStream_t s);
+                               int64_t B, int64_t Hkv, int64_t max_len, int64_t keep, int64_t recent, hipStream_t s);
 // Moves the kept rows of up to 3 tensors (B, Hkv, cap) together, through scratch (B, Hkv, keep); zeroed: the
 // one (4-byte rows) whose places left behind become zero, or -1.
 struct gt_kv_moved {

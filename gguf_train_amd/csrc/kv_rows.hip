@@ -3,9 +3,11 @@
 //
 // Choosing (kv_select_kernel): per sequence and kv head, the `recent` last tokens and the `keep - recent`
 // others of the largest weights, the lowest index of equal ones, in order.  A workgroup finds the smallest
-// weight that stays by radix selection, 8 bits of the order-preserving integer form of the floats a pass (four
-// passes over 4 bytes a token, from the caches after the first), and then walks the tokens in order, each
-// wavefront's places from ballots.  Integer counts alone decide, so the result does not depend on timing.
+// weight that stays by radix selection, 8 bits of the order-preserving integer form of the floats a pass, and then
+// gives those that stay their places in order, from ballots and a scan of their counts.  Up to kSelectCached tokens
+// a thread keeps its weights in registers and one scan serves them all, more are read again from the caches, 1024
+// tokens a scan.  Bound: latency, the passes' barriers and counting (LDS atomics), not the 4 bytes a token.  Integer
+// counts alone decide, so the result does not depend on timing.
 //
 // Moving, HBM-bound: the rows that change place go to scratch memory and from there to their new places, two
 // launches; writing them in place would have workgroups overwrite rows that others have yet to read.
@@ -16,7 +18,8 @@
 
 namespace {
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectKeys = 8;  // keys a thread keeps
+constexpr int kSelectCached = kSelectThreads * kSelectKeys;
 
 // Unsigned integers in the order of the floats: -0 as +0, every NaN above all others.
 __device__ inline uint32_t order_of(float x) {
@@ -35,6 +38,8 @@ struct SelectArgs {
     int Hkv, keep, recent;
 };
 
+// CACHED: no sequence has more than kSelectCached tokens.
+template <bool CACHED>
 __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a) {
     constexpr int WAVES = kSelectThreads / 64, COPIES = 4;
     __shared__ uint32_t s_hist[COPIES][256];
@@ -56,14 +61,31 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a)
     const int others = n - a.recent, m = a.keep - a.recent;  // 0 <= m < others
     for (int i = tid; i < a.recent; i += kSelectThreads) kept[m + i] = others + i;
     if (m == 0) return;
+    uint32_t keys[CACHED ? kSelectKeys : 1];
+    if constexpr (CACHED) {
+        float x[kSelectKeys];
+#pragma unroll
+        for (int c = 0; c < kSelectKeys; ++c) x[c] = w[min(tid + c * kSelectThreads, others - 1) * a.ws];
+#pragma unroll
+        for (int c = 0; c < kSelectKeys; ++c) keys[c] = order_of(x[c]);
+    }
+    // visit(key) for every token of this thread
+    auto each = [&](auto &&visit) {
+        if constexpr (CACHED) {
+#pragma unroll
+            for (int c = 0; c < kSelectKeys; ++c)
+                if (tid + c * kSelectThreads < others) visit(keys[c]);
+        } else {
+            for (int i = tid; i < others; i += kSelectThreads) visit(order_of(w[i * a.ws]));
+        }
+    };
     uint32_t prefix = 0, mask = 0, need = (uint32_t)m;
     for (int shift = 24; shift >= 0; shift -= 8) {
         for (int i = tid; i < COPIES * 256; i += kSelectThreads) (&s_hist[0][0])[i] = 0;
         __syncthreads();
-        for (int i = tid; i < others; i += kSelectThreads) {
-            const uint32_t k = order_of(w[i * a.ws]);
+        each([&](uint32_t k) {
             if ((k & mask) == prefix) atomicAdd(&s_hist[wv % COPIES][(k >> shift) & 255], 1u);
-        }
+        });
         __syncthreads();
         if (wv == 0) {
             // bins 255 - 4 lane downwards; the bin in which the count from the top reaches `need`
@@ -96,9 +118,7 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a)
     }
     // tokens above the border all stay, and the first `need` of those on it
     int above = 0, equal = 0;  // of the tokens before this chunk
-    for (int i0 = 0; i0 < others; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        const uint32_t k = i < others ? order_of(w[i * a.ws]) : 0u;
+    auto chunk = [&](int i, uint32_t k) {
         const bool up = i < others && k > prefix, eq = i < others && k == prefix;
         const uint64_t bu = __ballot(up), be = __ballot(eq);
         if (lane == 0) {
@@ -120,6 +140,44 @@ __global__ __launch_bounds__(kSelectThreads) void kv_select_kernel(SelectArgs a)
         pe += __popcll(be & lower);
         if (up || (eq && pe < (int)need)) kept[pu + min(pe, (int)need)] = i;
         __syncthreads();
+    };
+    if constexpr (CACHED) {
+        // counts of every 64 tokens: above the border in the low half, on it in the high half (each below 2^16)
+        __shared__ uint32_t s_count[kSelectKeys * WAVES];
+        static_assert(kSelectKeys * WAVES == 128, "two counts a lane");
+        uint64_t bu[kSelectKeys], be[kSelectKeys];
+#pragma unroll
+        for (int c = 0; c < kSelectKeys; ++c) {
+            const bool there = tid + c * kSelectThreads < others;
+            bu[c] = __ballot(there && keys[c] > prefix);
+            be[c] = __ballot(there && keys[c] == prefix);
+            if (lane == 0) s_count[c * WAVES + wv] = (uint32_t)__popcll(bu[c]) | (uint32_t)__popcll(be[c]) << 16;
+        }
+        __syncthreads();
+        if (wv == 0) {
+            const uint32_t x0 = s_count[2 * lane], x1 = s_count[2 * lane + 1];
+            uint32_t upto = x0 + x1;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += y;
+            }
+            s_count[2 * lane] = upto - x1 - x0;
+            s_count[2 * lane + 1] = upto - x1;
+        }
+        __syncthreads();
+        const uint64_t lower = (1ull << lane) - 1;
+#pragma unroll
+        for (int c = 0; c < kSelectKeys; ++c) {
+            const uint32_t before = s_count[c * WAVES + wv];
+            const int pu = (int)(before & 0xffffu) + __popcll(bu[c] & lower), pe = (int)(before >> 16) + __popcll(be[c] & lower);
+            const bool up = bu[c] >> lane & 1, eq = be[c] >> lane & 1;
+            if (up || (eq && pe < (int)need)) kept[pu + min(pe, (int)need)] = tid + c * kSelectThreads;
+        }
+    } else {
+        for (int i0 = 0; i0 < others; i0 += kSelectThreads) {
+            const int i = i0 + tid;
+            chunk(i, i < others ? order_of(w[i * a.ws]) : 0u);
+        }
     }
 }
 
@@ -215,10 +273,12 @@ hipError_t launch_rows_read(const void *k, const void *v, const int32_t *len, vo
 }  // namespace
 
 hipError_t gt_launch_kv_select(const float *w, const int64_t *strides, const int32_t *len, int32_t *next, int32_t *evicted, int64_t *kept,
-                               int64_t B, int64_t Hkv, int64_t keep, int64_t recent, hipStream_t s) {
+                               int64_t B, int64_t Hkv, int64_t max_len, int64_t keep, int64_t recent, hipStream_t s) {
     SelectArgs a{w, strides[0], strides[1], strides[2], len, next, evicted, kept, (int)Hkv, (int)keep, (int)recent};
     if (B * Hkv > 0x7fffffff) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(kv_select_kernel, dim3((unsigned)(B * Hkv)), dim3(kSelectThreads), 0, s, a);
+    const dim3 grid((unsigned)(B * Hkv));
+    if (max_len <= kSelectCached) hipLaunchKernelGGL(kv_select_kernel<true>, grid, dim3(kSelectThreads), 0, s, a);
+    else hipLaunchKernelGGL(kv_select_kernel<false>, grid, dim3(kSelectThreads), 0, s, a);
     return hipGetLastError();
 }
 

@@ -101,7 +101,7 @@ def tokens(c):
 
 @pytest.mark.parametrize("kind", CACHES)
 @pytest.mark.parametrize("B,Hkv,T,D,keep,recent", [(2, 3, 200, 64, 100, 10), (1, 1, 33, 128, 1, 0), (1, 2, 300, 96, 299, 0), (2, 1, 2500, 64, 1000, 1000),
-                                                   (1, 4, 64, 256, 32, 31), (1, 1, 1500, 32, 7, 3)])
+                                                   (1, 4, 64, 256, 32, 31), (1, 1, 1500, 32, 7, 3), (1, 2, 9001, 32, 700, 9)])
 def test_evict(dev, kind, B, Hkv, T, D, keep, recent):
     k, v = randn((B, Hkv, T, D), 20, torch.float16), randn((B, Hkv, T, D), 21, torch.float16)
     c = make(dev, k, v, kind, cap=T + 40)
