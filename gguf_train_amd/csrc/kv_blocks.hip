@@ -141,22 +141,17 @@ struct RowSource {
     }
 };
 
-// The V codes of a few units in LDS, 16 dims at a pitch that puts a wavefront's bytes, 16 apart, into different banks
-// two by two.
-constexpr int kStagedUnits = 3, kStagedPitch = 1024 + 8;
-
 // Tokens of another block cache (z 0 keys, 1 values): token `first` + i of the new cache is kept[i], in LDS.  A
-// token's V codes are 16 bytes apart, so that a wavefront's 64 take 16 lines of which the others hold other tokens':
-// STAGED, the units of all the workgroup's tokens are in LDS, from unit `unit0` on (columns only).
-template <bool E4M3, bool STAGED>
+// token's V codes are 16 bytes apart, so that a wavefront's 64 take 16 lines of which the others hold other tokens'.
+// The caches take care of that: with the units copied to LDS first, int8 D128 B4 Hkv8 4096 to 2048 tokens took 57.5
+// us with the append before it, without 55.3.
+template <bool E4M3>
 struct KeptSource {
     const uint8_t *codes;
     const float *scales, *tail;
     const int *kept;
     int first, here, full, shift, D, Dp, z;  // here: places of kept
     bool late;  // some of the workgroup's tokens are in the old tail
-    const uint8_t *staged;
-    int unit0;
     struct Dims {
         uint32_t w[4];
         float s;
@@ -192,19 +187,12 @@ struct KeptSource {
     // (past the workgroup's tokens: its last)
     __device__ int token(int t, int e) const { return __builtin_amdgcn_readfirstlane(kept[min(t + 16 * (e >> 2) + (e & 3) - first, here - 1)]); }
     __device__ void load(Column &r, int t, int d) const {
-        const uint32_t at = (uint32_t)((d >> 4) * (STAGED ? kStagedPitch : 1024) + (d & 15) * 16);
+        const uint32_t at = (uint32_t)((d >> 4) * 1024 + (d & 15) * 16);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int u = token(t, e);
-            if constexpr (STAGED) {
-                const int uc = u < full && u >= unit0 * kUnit ? u : unit0 * kUnit;
-                r.q[e] = staged[((uc >> 6) - unit0) * (Dp / 16) * kStagedPitch + (int)v_at(uc & 63, 0, Dp) + (int)at];
-                r.s[e] = scales[uc >> shift];
-            } else {
-                const int uc = u < full ? u : 0;
-                r.q[e] = (codes + v_at(uc, 0, Dp))[at];
-                r.s[e] = scales[uc >> shift];
-            }
+            const int u = token(t, e), uc = u < full ? u : 0;
+            r.q[e] = (codes + v_at(uc, 0, Dp))[at];
+            r.s[e] = scales[uc >> shift];
         }
     }
     __device__ void values(const Column &r, int t, int d, float *v) const {
@@ -331,24 +319,21 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int shif
 
 // The tokens after the last whole block, from token `from` of the cache on (those before are there): their values,
 // and the operands that the attention takes them as (the row divided by its own power of two, float16 hi + lo, in
-// the codes' order).  First DP / 16 lanes a row, for its largest magnitude; K's operands are written there.  V's
-// lie with 16 tokens of a dim together: a few rows are written an element at a time, more (32 bytes a lane: a prompt's
-// tail of 17 rows took 14 us otherwise) from a second look at the tokens of the tail, the old ones among them.  clear:
-// the operands of tokens to come become zeros.
+// the codes' order).  DP / 16 lanes a row, for its largest magnitude.  V's operands, 32 bytes apart, are written an element
+// at a time; a second pass that wrote them 16 tokens of a dim together was slower up to 64 rows (B4 Hkv8 D128: 17 rows
+// of a block of 32 6.5 against 5.6 us, 100 of a block of 128 12.6 against 14.3).  clear: the operands of tokens to come
+// become zeros.
 template <int DP, typename Source>
 __device__ inline void append_tail(const Source &src, const Side &to, int shift, int D, int z, int from, int total, bool clear) {
     constexpr int CH = DP / 16;
-    __shared__ float s_inv[kMaxBlock];  // a token's scale, inverted (0: not a finite row)
-    const int whole = total >> shift << shift, room = max(1 << shift, kUnit), rows = total - from;
-    const bool columns = z == 1 && rows > 4;
+    const int whole = total >> shift << shift, room = max(1 << shift, kUnit);
     const int64_t plane = (int64_t)room * DP;
-    const int first = columns ? whole : from;
     if (clear) {
         for (int i = threadIdx.x; i < (int)(plane / 4); i += kThreads) ((uint4 *)to.ops)[i] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
     }
-    for (int i = threadIdx.x; i < (total - first) * CH; i += kThreads) {
-        const int p = first + i / CH, t = p - whole, d0 = i % CH * 16;
+    for (int i = threadIdx.x; i < (total - from) * CH; i += kThreads) {
+        const int p = from + i / CH, t = p - whole, d0 = i % CH * 16;
         float v[16];
         typename Source::Dims raw;
         src.load(raw, p, d0);
@@ -360,24 +345,18 @@ __device__ inline void append_tail(const Source &src, const Side &to, int shift,
         const bool bad = most >= 0x7f800000u;
         const int e2 = bad || most == 0 ? -126 : min(max((int)(most >> 23) - 127, -126), 126);
         const float f = bad ? 0.0f : __uint_as_float((uint32_t)(127 - e2) << 23);
-        if (d0 == 0) {
-            to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
-            s_inv[t] = f;
-        }
-        if (p >= from) {
-            float *row = to.tail + (int64_t)t * D + d0;
-            if (D % 16 == 0) {
-                if (d0 < D) {
+        if (d0 == 0) to.op_scales[t] = bad ? NAN : __uint_as_float((uint32_t)(127 + e2) << 23);
+        float *row = to.tail + (int64_t)t * D + d0;
+        if (D % 16 == 0) {
+            if (d0 < D) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) ((float4 *)row)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (d0 + e < D) row[e] = v[e];
+                for (int e = 0; e < 4; ++e) ((float4 *)row)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
             }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (d0 + e < D) row[e] = v[e];
         }
-        if (columns) continue;
         typedef _Float16 half8 __attribute__((ext_vector_type(8)));
         half8 hi[2], lo[2];
 #pragma unroll
@@ -399,30 +378,6 @@ __device__ inline void append_tail(const Source &src, const Side &to, int shift,
                 o[plane + 16 * e] = lo[e >> 3][e & 7];
             }
         }
-    }
-    if (!columns) return;
-    __syncthreads();
-    for (int i = threadIdx.x; i < room / 16 * DP; i += kThreads) {
-        const int t = __builtin_amdgcn_readfirstlane(i / (4 * DP) * kUnit + 4 * (i / DP % 4)), d = i % DP;  // + 16 kb + r
-        if (whole + t >= total) continue;
-        float v[16];
-        typename Source::Column raw;
-        src.load(raw, whole + t, d);
-        src.values(raw, whole + t, d, v);
-        typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-        half8 hi[2], lo[2];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int at = t + 16 * (e >> 2) + (e & 3);
-            const float f = whole + at < total ? s_inv[at] : 0.0f;
-            const float y = f == 0.0f ? 0.0f : v[e] * f;
-            hi[e >> 3][e & 7] = (_Float16)y;
-            lo[e >> 3][e & 7] = (_Float16)(y - (float)hi[e >> 3][e & 7]);
-        }
-        half8 *o = (half8 *)(to.ops + v_at(t, d, DP));
-        o[0] = hi[0], o[1] = hi[1];
-        o = (half8 *)(to.ops + plane + v_at(t, d, DP));
-        o[0] = lo[0], o[1] = lo[1];
     }
 }
 
@@ -475,25 +430,9 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_evict_kernel(AppendArgs a)
     const Side from = slice<DP>(a.from[z], a, bg), to = slice<DP>(a.to[z], a, bg);
     const int whole = total >> a.shift << a.shift;
     const bool last = total - t0 <= NT;  // the tail's tokens are among the last workgroup's, or there are none
-    auto write = [&](const auto &src) {
-        append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
-        if (last) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
-    };
-    // the tokens are in order: their units
-    const int unit0 = s_kept[0] >> 6, units = (min(s_kept[max(min(NT, total - t0), 1) - 1], full - 1) >> 6) - unit0 + 1;
-    if (z == 1 && !last && units >= 1 && units <= kStagedUnits) {
-        __shared__ __attribute__((aligned(16))) uint8_t s_codes[kStagedUnits * (DP / 16) * kStagedPitch];
-        for (int i = threadIdx.x; i < units * 4 * DP; i += kThreads) {
-            const uint4 w = *(const uint4 *)(from.codes + (int64_t)unit0 * kUnit * DP + 16 * i);
-            uint2 *o = (uint2 *)(s_codes + i / 64 * kStagedPitch + i % 64 * 16);
-            o[0] = make_uint2(w.x, w.y);
-            o[1] = make_uint2(w.z, w.w);
-        }
-        __syncthreads();
-        write(KeptSource<E4M3, true>{from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late, s_codes, unit0});
-    } else {
-        write(KeptSource<E4M3, false>{from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late, nullptr, 0});
-    }
+    const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late};
+    append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
+    if (last) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
 }
 
 struct ReadArgs {
