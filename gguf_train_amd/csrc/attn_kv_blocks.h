@@ -1,5 +1,5 @@
-// Attention of few query rows over the 8-bit block cache (kv_blocks.h), straight from the codes: decode steps,
-// and the several tokens of a draft that are checked together.
+// Attention over the 8-bit block cache (kv_blocks.h), straight from the codes: decode steps, the several tokens of a
+// draft that are checked together, and prompts that are too short to fill the GPU otherwise.
 //
 //   s[r, t] = scale q_r . k_t,  p = softmax over the keys that row r sees,  o_r = sum_t p[r, t] v_t
 // with k_t = code x 2^a, v_t = code x 2^c, a and c a block's exponents.  HBM-bound: K and V are read once, a
@@ -270,10 +270,17 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
     const int64_t x = blockIdx.x, slices = (int64_t)a.B * a.Hkv, bg = x % slices, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
     const int rg = (int)(x / slices), G = a.H / a.Hkv, rows = G * a.L;
     const int r0 = rg * kColumns, nr = min(kColumns, rows - r0);
-    const int len = a.len[b], full = len >> a.shift << a.shift, tail = len - full;
+    const int len = a.len[b], full = len >> a.shift << a.shift;
+    // keys from `seen` on are seen by no row of the group (with few tokens that is less than a unit)
+    int seen = len;
+    if (a.causal && a.L > kUnit) {
+        const int h0 = r0 / a.L, last = r0 + nr - 1;
+        seen = len - a.L + (last >= (h0 + 1) * a.L ? a.L : last - h0 * a.L + 1);
+    }
+    const int tail = min(len, seen) - full;
 
     // ---- whole blocks: the first unit's loads are on their way while the queries are made ready ----
-    const int u0 = blockIdx.y * a.span, u1 = min(u0 + a.span, (full + kUnit - 1) / kUnit);
+    const int u0 = blockIdx.y * a.span, held = min(u0 + a.span, (full + kUnit - 1) / kUnit), u1 = min(held, (seen + kUnit - 1) / kUnit);
     const int64_t from = (bg * a.units + u0) * kUnit * Dp;
     // buffer loads: a uniform place, a lane's 16 bytes; past the last unit they return zeros and fetch nothing
     const int bytes = max(u1 - u0, 0) * kUnit * Dp;  // (below 2^31: gt_kv_blocks_attn_supported)
@@ -424,8 +431,8 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
     }
 
     // ---- the tail: by the last split that has units, as its next ones ----
-    const int nu = max(u1 - u0, 0);
-    const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && u1 * kUnit >= full;
+    const int nu = max(held - u0, 0);
+    const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && held * kUnit >= full;
     const int room = max(1 << a.shift, kUnit);  // tokens of a plane of operands
     for (int tu = 0; mine && tu * kUnit < tail; ++tu) {
         if ((nu + tu) % kWaves != w) continue;

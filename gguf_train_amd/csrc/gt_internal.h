@@ -192,9 +192,8 @@ hipError_t gt_launch_kv_blocks_evict(const gt_kv_blocks &from, const gt_kv_block
 // that are not held.
 hipError_t gt_launch_kv_blocks_read(const gt_kv_blocks &c, const int32_t *len, int64_t rows, void *k, void *v, int dtype,
                                     hipStream_t s);
-// Attention of few rows over the block cache (attn_kv_blocks.h): q (B, H, L, D) with contiguous dims, o dense of
+// Attention over the block cache (attn_kv_blocks.h): q (B, H, L, D) with contiguous dims, o dense of
 // q's dtype, lse (B, H, L) or null.  `note` describes the launch.
-constexpr int64_t kKvBlocksAttnRows = 128;
 struct gt_kv_blocks_attn {
     const void *q;
     void *o;

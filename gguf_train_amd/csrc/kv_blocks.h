@@ -35,7 +35,6 @@ constexpr int kMaxDim = 256;
 constexpr int kMaxBlock = 128;
 
 GT_KVB_FN inline int padded_dim(int64_t D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
-GT_KVB_FN inline int64_t padded_tokens(int64_t cap) { return (cap + kUnit - 1) / kUnit * kUnit; }
 
 // Byte of (token t, dim d) in the codes of one sequence and head.
 GT_KVB_FN inline int64_t k_at(int64_t t, int d, int Dp) {

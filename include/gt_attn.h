@@ -410,9 +410,9 @@ GT_API gt_tensor *gt_kv_cache_attention(gt_kv_cache *c, const gt_tensor *q, floa
  * the tokens were appended.  A block with an infinity or NaN reads as NaN.  head_dim up to 256 (storage is
  * padded to 64, 128 or 256), batch * n_head_kv up to 65535.  The gt_kv_cache_* entry points take it like any
  * other cache, but for gt_kv_cache_keys / values, which fail (gt_kv_cache_read gives the values); float64 rows
- * are rounded to float32.  Attention is computed on the values: float32, float16 and bfloat16 queries of up to
- * 128 rows per kv head (H / n_head_kv * L) straight from the codes; other calls read the values into a
- * temporary first, in the queries' dtype if every token was appended in it, else in float32. */
+ * are rounded to float32.  Attention is computed on the values, straight from the codes; float64 queries, and
+ * float16 and bfloat16 queries of so many rows that it is faster, read the values into a temporary first, in the
+ * queries' dtype if every token was appended in it, else in float32. */
 GT_API gt_kv_cache *gt_kv_cache_create_blocks(int64_t batch, int64_t n_head_kv, int64_t capacity, int64_t head_dim,
                                               int dtype, int block_tokens, int device_index);
 /* The values a cache of any dtype stands for: new device tensors (batch, n_head_kv, longest length, head_dim)
