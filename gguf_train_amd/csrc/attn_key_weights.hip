@@ -36,7 +36,8 @@ struct Args {
     const float *lse;
     const int32_t *len;
     float *sums;   // (B, Hkv, cap)
-    float *parts;  // (splits, B, Hkv, cap), or null: one split writes sums
+    float *parts;  // (splits, B, Hkv, max_len), or null: one split writes sums
+    int64_t max_len;
     float keep;
     float scale;
     int causal, q_vec, k_dtype;
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
             for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o, 64);
             const int t = k0 + 16 * kb + 4 * g + i;
             if (n != 0 || t >= len) continue;
-            if (a.parts) a.parts[((int64_t)blockIdx.z * gridDim.y + bg) * a.cap + t] = s;
+            if (a.parts) a.parts[((int64_t)blockIdx.z * gridDim.y + bg) * a.max_len + t] = s;
             else {
                 float *o = a.sums + bg * a.cap + t;
                 *o = a.keep == 0.0f ? s : fmaf(a.keep, *o, s);
@@ -241,12 +242,12 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
         }
 }
 
-__global__ void add_parts_kernel(const float *parts, int splits, int64_t stride, const int32_t *len, float *sums, float keep,
+__global__ void add_parts_kernel(const float *parts, int splits, int64_t max_len, const int32_t *len, float *sums, float keep,
                                  int Hkv, int64_t cap) {
     const int64_t bg = blockIdx.y, t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (t >= len[bg / Hkv]) return;
     float s = 0.0f;
-    for (int z = 0; z < splits; ++z) s += parts[z * stride + bg * cap + t];
+    for (int z = 0; z < splits; ++z) s += parts[((int64_t)z * gridDim.y + bg) * max_len + t];
     float *o = sums + bg * cap + t;
     *o = keep == 0.0f ? s : fmaf(keep, *o, s);
 }
@@ -325,13 +326,14 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
     splits = (tiles + a.span - 1) / a.span;
     gt_scratch parts;
     if (splits > 1) {
-        if (!gt_scratch_alloc(parts, (size_t)(splits * r.B * r.Hkv * r.cap) * sizeof(float), dev)) return hipErrorOutOfMemory;
+        if (!gt_scratch_alloc(parts, (size_t)(splits * r.B * r.Hkv * r.max_len) * sizeof(float), dev)) return hipErrorOutOfMemory;
         a.parts = (float *)parts.ptr();
+        a.max_len = r.max_len;
     }
     void *args[] = {(void *)&a};
     hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)wgs, (unsigned)(r.B * r.Hkv), (unsigned)splits), dim3(64 * kWaves), args, 0, s);
     if (e != hipSuccess || splits == 1) return e;
     hipLaunchKernelGGL(add_parts_kernel, dim3((unsigned)((r.max_len + 255) / 256), (unsigned)(r.B * r.Hkv)), dim3(256), 0, s,
-                       (const float *)a.parts, (int)splits, r.B * r.Hkv * r.cap, r.len, r.sums, r.keep, (int)r.Hkv, r.cap);
+                       (const float *)a.parts, (int)splits, r.max_len, r.len, r.sums, r.keep, (int)r.Hkv, r.cap);
     return hipGetLastError();
 }

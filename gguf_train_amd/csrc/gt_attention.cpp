@@ -1357,6 +1357,11 @@ struct KvBlockMemory {
         for (int i = 0; i < 2; ++i)
             for (gt_tensor *t : {codes[i], scales[i], tail[i], ops[i], op_scales[i]}) gt_tensor_free(t);
     }
+    // Once freed, the memory is given to allocations for this stream only.
+    void last_used_on(hipStream_t s) {
+        for (int i = 0; i < 2; ++i)
+            for (gt_tensor *t : {codes[i], scales[i], tail[i], ops[i], op_scales[i]}) t->storage->stream = s;
+    }
     void swap(KvBlockMemory &o) {
         for (int i = 0; i < 2; ++i) {
             std::swap(codes[i], o.codes[i]);
@@ -2118,7 +2123,10 @@ int kv_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weig
                            "kv cache block evict kernel")) &&
              gt_hip_check(gt_launch_kv_move(moved, n, zeroed, places, len, B, Hkv, keep, max_len, c->cap, gt_stream()), "kv cache move kernel");
         if (ok) {
-            if (c->block) c->mem.swap(next);
+            if (c->block) {
+                c->mem.swap(next);
+                next.last_used_on(gt_stream());  // this stream's kernels read it, whichever it was made on
+            }
             std::swap(c->len_dev, c->len_next);
             for (auto &x : c->len) x = (int32_t)std::min<int64_t>(x, keep);
         }

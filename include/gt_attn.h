@@ -436,8 +436,9 @@ GT_API gt_tensor *gt_kv_cache_weights(gt_kv_cache *c);
  * tokens and the keep - recent others of the largest weights (the earliest of equal ones; a NaN counts as the
  * largest), in their order.  weights: float (batch, n_head_kv, at least the longest length), NULL for the
  * accumulated ones; those of the tokens that stay, stay with them.  A block cache's tokens are quantized again
- * in their new blocks (exactly, unless their scale grows).  kept (NULL: not wanted) receives a new device tensor
- * (batch, n_head_kv, keep) int64, the index each kept token had, -1 past a shorter sequence's length.
+ * in their new blocks (exactly, unless their scale grows), in new memory of the cache's size.  kept (NULL: not
+ * wanted) receives a new device tensor (batch, n_head_kv, keep) int64, the index each kept token had, -1 past a
+ * shorter sequence's length.
  * Positions go on from what was appended, not from the length: gt_kv_cache_position, pos_offset and the
  * angles of gt_kv_cache_append_rope count evicted tokens.  Keys are kept as they were appended (rotated). */
 GT_API int gt_kv_cache_evict(gt_kv_cache *c, int64_t keep, int64_t recent, const gt_tensor *weights, gt_tensor **kept);

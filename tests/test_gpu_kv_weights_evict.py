@@ -260,6 +260,57 @@ def test_other_stream(dev):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("kind", CACHES)
+def test_memory_of_an_eviction_on_another_stream_is_not_given_away(dev, kind):
+    """What a cache of one stream held is read by an eviction that waits on another, while the first goes on."""
+    k, v = randn((2, 2, 500, 64), 90, torch.float16), randn((2, 2, 500, 64), 91, torch.float16)
+    w = torch.rand(2, 2, 500, generator=torch.Generator().manual_seed(92))
+    plain = make(dev, k, v, kind)
+    plain.evict(100, 10, w.to(dev))
+    want = plain.read()
+    side = torch.cuda.Stream(dev)
+    c, wd, other = make(dev, k, v, kind), w.to(dev), [torch.randn(2, 2, 500, 64, device=dev, dtype=torch.float16) for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)  # (some milliseconds)
+        c.evict(100, 10, wd)
+    later = [g.KVCache(2, 2, 500, 64, kind, dev) for _ in range(3)]
+    for x in later:
+        x.append(*other)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(c.read(), want))
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_many_rows_over_few_tokens_of_a_large_cache(dev, kind):
+    """Sums from several column splits, whose parts take the room of the tokens held, not of the capacity."""
+    k, v, q = (randn((1, 2, 90, 64), 93 + i, torch.float16) for i in range(3))
+    q = randn((1, 32, 90, 64), 96, torch.float16)
+    c = make(dev, k, v, kind, cap=200_000)
+    c.attention(q.to(dev), accumulate=1.0)
+    weight_checks(c, c.weights()[..., :1000], q, torch.zeros((1, 2, 90), dtype=torch.float64), 0.0, True, "large")
+    assert c.weights()[..., 90:].abs().max().item() == 0.0
+
+
+@pytest.mark.parametrize("kind", CACHES)
+def test_nothing_to_evict_and_a_full_cache(dev, kind):
+    k, v = randn((1, 2, 96, 64), 97, torch.float16), randn((1, 2, 96, 64), 98, torch.float16)
+    c = make(dev, k[:, :, :70], v[:, :, :70], kind, cap=96)
+    before = c.read()
+    kept = c.evict(96, 0, torch.rand(1, 2, 70, device=dev))
+    assert kept.tolist() == [[list(range(70)) + [-1] * 26] * 2] and c.lengths == [70] and c.position() == 70
+    assert all(torch.equal(a, b) for a, b in zip(c.read(), before))
+    c.append(k[:, :, 70:].to(dev), v[:, :, 70:].to(dev))  # to the last token of the capacity
+    whole = make(dev, k, v, kind)
+    assert all(torch.equal(a, b) for a, b in zip(c.read(), whole.read()))
+    q = randn((1, 4, 1, 64), 99, torch.float16).to(dev)
+    assert torch.equal(c.attention(q), whole.attention(q))
+    with pytest.raises(RuntimeError, match="do not fit"):
+        c.append(k[:, :, :1].to(dev), v[:, :, :1].to(dev))
+    assert c.evict(1, 1, torch.rand(1, 2, 96, device=dev)).tolist() == [[[95], [95]]] and c.lengths == [1] and c.position() == 96
+    assert torch.equal(c.read()[0][:, :, 0].half().cpu(), whole.read()[0][:, :, 95].half().cpu())
+
+
 def test_refusals(dev):
     c = g.KVCache(1, 2, 50, 64, torch.int8, dev)
     k = torch.ones((1, 2, 40, 64), device=dev)
