@@ -282,26 +282,28 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
     // ---- whole blocks: the first unit's loads are on their way while the queries are made ready ----
     const int u0 = blockIdx.y * a.span, held = min(u0 + a.span, (full + kUnit - 1) / kUnit), u1 = min(held, (seen + kUnit - 1) / kUnit);
     const int64_t from = (bg * a.units + u0) * kUnit * Dp;
-    // buffer loads: a uniform place, a lane's 16 bytes; past the last unit they return zeros and fetch nothing
-    const int bytes = max(u1 - u0, 0) * kUnit * Dp;  // (below 2^31: gt_kv_blocks_attn_supported)
-    const auto kr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.k + from), 0, bytes, 0x00027000);
-    const auto vr = __builtin_amdgcn_make_buffer_rsrc((void *)(a.v + from), 0, bytes, 0x00027000);
+    // buffer loads of a unit each, a lane's 16 bytes: past the last unit the buffer is empty, they return zeros and fetch
+    // nothing.  (Places are in the buffer's address and the lanes' offsets: a uniform offset is not checked.)
+    auto buffer = [&](const uint8_t *codes, int u) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)(codes + from + (int64_t)(u - u0) * (kUnit * Dp)), 0, u < u1 ? kUnit * Dp : 0, 0x00027000);
+    };
     const int64_t nblk = a.units * kUnit >> a.shift;
     const float *sc = ((lane & 4) ? a.vs : a.ks) + bg * nblk;  // lanes 0..3 hold K's scales, 4..7 V's
     u32x4 rk[DT], rv[DT];
     float rs = 0.0f;
     constexpr int kNonTemporal = 2;
-    auto load_k = [&](int u) {
+    auto load_unit = [&](u32x4 *to, const uint8_t *codes, int u) {
+        const auto r = buffer(codes, u);
+        int at = 16 * lane;
+        asm volatile("" : "+v"(at));  // (the offsets are not kept in registers from unit to unit)
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-            rk[t] = __builtin_amdgcn_raw_buffer_load_b128(kr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
+        for (int t = 0; t < DT; ++t) to[t] = __builtin_amdgcn_raw_buffer_load_b128(r, at + 1024 * t, 0, kNonTemporal);
+    };
+    auto load_k = [&](int u) {
+        load_unit(rk, a.k, u);
         rs = sc[min((u * kUnit + 16 * (lane & 3)) >> a.shift, (int)nblk - 1)];
     };
-    auto load_v = [&](int u) {
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-            rv[t] = __builtin_amdgcn_raw_buffer_load_b128(vr, 16 * lane, (u - u0) * kUnit * Dp + 1024 * t, kNonTemporal);
-    };
+    auto load_v = [&](int u) { load_unit(rv, a.v, u); };
     if (u0 + w < u1) {
         load_k(u0 + w);
         load_v(u0 + w);

@@ -43,10 +43,10 @@ int64_t resident_groups(const void *kernel) {
 // groups) 57 against 90, 2048 rows 100 against 91; B4 Hkv8 S512 256 rows 13.7 against 21.7, 1024 rows 37 against 24;
 // B1 Hkv2 S16384 4096 rows (512 groups) 169 against 302.  float32 queries and more than 128 dims have no such fast
 // path (D128 B16 Hkv8 S2048 64 rows float32 39 against 567, D256 B8 Hkv8 S4096 512 rows 487 against 49550).
-bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int64_t max_len, int q_dtype) {
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype) {
     const int64_t rows = H / c.Hkv * L, groups = c.B * c.Hkv * ((rows + kColumns - 1) / kColumns);
     const bool better = rows <= 128 || groups <= 512 || q_dtype == GT_F32 || c.Dp > 128;
-    return (q_dtype == GT_F16 || q_dtype == GT_BF16 || q_dtype == GT_F32) && better && c.B * H * L < (1LL << 31) && (max_len + kUnit) * c.Dp < (1LL << 31);  // (32-bit offsets)
+    return (q_dtype == GT_F16 || q_dtype == GT_BF16 || q_dtype == GT_F32) && better && c.B * H * L < (1LL << 31);
 }
 
 hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note) {

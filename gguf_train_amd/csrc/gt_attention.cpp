@@ -1858,7 +1858,7 @@ gt_tensor *kv_attention(gt_kv_cache *c, const gt_tensor *q, float scale, int is_
     int q8 = 0;
     if (c->block && o->numel > 0) {
         const gt_kv_blocks blocks = kv_blocks_of(c, c->mem);
-        if (gt_kv_blocks_attn_supported(blocks, H, L, maxlen, q->dtype)) {
+        if (gt_kv_blocks_attn_supported(blocks, H, L, q->dtype)) {
             const gt_tensor *qs = stage(q, dev, q->dtype, tmp);
             ok = qs != nullptr;
             if (ok) {

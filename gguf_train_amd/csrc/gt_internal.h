@@ -203,7 +203,7 @@ struct gt_kv_blocks_attn {
     int q_dtype, causal;
     float scale;
 };
-bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int64_t max_len, int q_dtype);
+bool gt_kv_blocks_attn_supported(const gt_kv_blocks &c, int64_t H, int64_t L, int q_dtype);
 hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_attn &r, int dev, hipStream_t s, std::string &note);
 // Sums of the attention weights of a cache's tokens (attn_key_weights.hip): sums (B, Hkv, cap) becomes keep *
 // sums + the weights' sums over the rows of q and the heads of a group, from the attention's lse.  The keys:
