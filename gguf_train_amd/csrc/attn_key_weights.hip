@@ -21,6 +21,8 @@ namespace {
 
 using namespace gtkvb;
 
+constexpr int kWaves = 4;
+
 enum Source { kInt8, kE4m3, kF16, kBf16, kF32, kQ8, kAny };  // kAny: float rows not in whole aligned pieces of 16 dims
 
 struct Args {

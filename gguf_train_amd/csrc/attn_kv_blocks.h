@@ -9,7 +9,7 @@
 // instruction; more than 16 take further workgroups over the same keys (two or four tiles of columns in a
 // workgroup, which decode the keys once for all, left one wavefront per SIMD and took longer: D128 32 rows of S1024
 // 19 against 16.5 us, 128 rows of S4096 42 against 35).  A workgroup owns a span of 64-token units (a split of the
-// sequence), its four wavefronts take them in turn, each with its own running maximum and sum; they are joined
+// sequence), its wavefronts take them in turn, each with its own running maximum and sum; they are joined
 // once at the end, and the last split of a row group to finish joins the splits (partials in uncached memory, as
 // in decode_merge.h).
 //
@@ -51,7 +51,6 @@ using gtmfma::kLog2e;
 using gtmfma::u32x4;
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4;
 constexpr int kColumns = 16;  // rows of a workgroup
 
 struct AttnArgs {
@@ -192,16 +191,16 @@ __device__ inline float query_operands(const QueryRow<QT, NI> &q, const QT *row,
 // Joins the splits of rows row0 .. row0 + n - 1; uncached partials (see decode_merge.h), each load a round trip
 // to the memory: the (max, sum) pairs of all rows first, into LDS, then every thread four dims of a row, eight
 // splits in flight.  lds: n * nsplit floats.
-template <typename TO, int NI>
+template <typename TO, int NI, int W>
 __device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, float *lds) {
     constexpr int Dp = 64 * NI, PIECES = Dp / 4;
     __shared__ float s_inv[kColumns];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ns = a.nsplit;  // ns <= 64
-    constexpr int RW = kColumns / kWaves;
-    float mi[RW], li[RW];  // rows w, w + 4, ...: split `lane`
+    constexpr int RW = (kColumns + W - 1) / W;
+    float mi[RW], li[RW];  // rows w, w + W, ...: split `lane`
 #pragma unroll
     for (int k = 0; k < RW; ++k) {
-        const int r = w + kWaves * k;
+        const int r = w + W * k;
         const float *ml = a.part_ml + ((row0 + min(r, n - 1)) * ns + min(lane, ns - 1)) * 2;
         if (r < n) {
             mi[k] = lane < ns ? ml[0] : -INFINITY;
@@ -210,7 +209,7 @@ __device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, floa
     }
 #pragma unroll
     for (int k = 0; k < RW; ++k) {
-        const int r = w + kWaves * k;
+        const int r = w + W * k;
         if (r >= n) break;
         float M = mi[k];
         for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
@@ -225,7 +224,7 @@ __device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, floa
         }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < n * PIECES; e += 64 * kWaves) {
+    for (int e = threadIdx.x; e < n * PIECES; e += 64 * W) {
         const int r = e / PIECES, d = 4 * (e % PIECES);
         const float *po = a.part_o + (row0 + r) * ns * Dp + d;
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -249,18 +248,18 @@ __device__ inline void merge_splits(const AttnArgs &a, int64_t row0, int n, floa
 }
 
 // LDS of a launch: the wavefronts' rows on their way to being joined, or the splits' weights.
-GT_KVB_FN inline int64_t attn_lds_floats(int rows, int Dp, int nsplit) {
-    const int64_t join = 2 * (int64_t)rows * (Dp + 4), merge = (int64_t)rows * nsplit;
+GT_KVB_FN inline int64_t attn_lds_floats(int rows, int Dp, int nsplit, int waves) {
+    const int64_t join = waves / 2 * (int64_t)rows * (Dp + 4), merge = (int64_t)rows * nsplit;
     return join > merge ? join : merge;
 }
 
-template <typename QT, int NI, bool E4M3>
-__global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
+template <typename QT, int NI, bool E4M3, int W>
+__global__ __launch_bounds__(64 * W, NI <= 2 ? 2 : 1) void attn_kv_blocks_kernel(AttnArgs a) {
     constexpr bool F32 = __is_same(QT, float);
     constexpr int Dp = 64 * NI, DT = 4 * NI;
     constexpr int OP = Dp + 4;  // pitch of the rows to be joined
-    extern __shared__ __attribute__((aligned(16))) float s_o[];  // [2][row]
-    __shared__ float s_m[kWaves][kColumns], s_l[kWaves][kColumns];
+    extern __shared__ __attribute__((aligned(16))) float s_o[];  // [W / 2][row]
+    __shared__ float s_m[W][kColumns], s_l[W][kColumns], s_M[kColumns], s_L[kColumns];
     __shared__ int s_last;
 
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -424,12 +423,12 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
         }
     };
     // the next unit's K is on its way during the softmax and P.V, its V during the next scores
-    for (int u = u0 + w; u < u1; u += kWaves) {
+    for (int u = u0 + w; u < u1; u += W) {
         scores();
-        load_k(u + kWaves);
+        load_k(u + W);
         softmax(std::false_type{}, u * kUnit, full, [&](int kb, int) { return sk[kb]; }, [&](int kb, int) { return ev[kb]; });
         values();
-        load_v(u + kWaves);
+        load_v(u + W);
     }
 
     // ---- the tail: by the last split that has units, as its next ones ----
@@ -437,7 +436,7 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
     const bool mine = full == 0 ? blockIdx.y == 0 : nu > 0 && held * kUnit >= full;
     const int room = max(1 << a.shift, kUnit);  // tokens of a plane of operands
     for (int tu = 0; mine && tu * kUnit < tail; ++tu) {
-        if ((nu + tu) % kWaves != w) continue;
+        if ((nu + tu) % W != w) continue;
         const int t0 = tu * kUnit;
         const _Float16 *kt = a.kt + (bg * 2 * room + t0) * Dp + 16 * lane, *vt = a.vt + (bg * 2 * room + t0) * Dp + 16 * lane;
         const int64_t lo_at = (int64_t)room * Dp;
@@ -482,34 +481,44 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
         s_l[w][n] = lsum;
     }
     __syncthreads();
-    // waves 2 and 3 leave theirs, waves 0 and 1 add their own
+    if (threadIdx.x < kColumns) {
+        const int col = threadIdx.x;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int ww = 0; ww < W; ++ww) M = fmaxf(M, s_m[ww][col]);
+#pragma unroll
+        for (int ww = 0; ww < W; ++ww) {
+            const float lw = s_l[ww][col];
+            L += s_m[ww][col] == -INFINITY ? (lw != lw ? lw : 0.0f) : fast_exp2(s_m[ww][col] - M) * lw;
+        }
+        s_M[col] = M;
+        s_L[col] = L;
+    }
+    __syncthreads();
+    // the second half of the waves leave theirs, the first add their own
 #pragma unroll
     for (int half = 1; half >= 0; --half) {
-        if ((w >> 1) == half && n < nr) {
-            const float M = fmaxf(fmaxf(s_m[0][n], s_m[1][n]), fmaxf(s_m[2][n], s_m[3][n]));
+        if (w / (W / 2) == half && n < nr) {
+            const float M = s_M[n];
             const float to = mv == -INFINITY ? 0.0f : fast_exp2(mv - (M == -INFINITY ? 0.0f : M));
             const bool bad = lsum != lsum;
 #pragma unroll
             for (int t = 0; t < DT; ++t) {
                 f32x4 y = acc[t] * to;
                 if (bad) y = f32x4{NAN, NAN, NAN, NAN};
-                f32x4 *o = (f32x4 *)&s_o[((w & 1) * nr + n) * OP + 16 * t + 4 * g];
+                f32x4 *o = (f32x4 *)&s_o[(w % (W / 2) * nr + n) * OP + 16 * t + 4 * g];
                 *o = half == 0 ? *o + y : y;
             }
         }
         __syncthreads();
     }
     const int64_t row0 = (b * a.H + kvh * G) * a.L + r0;
-    for (int e = threadIdx.x; e < nr * Dp; e += 64 * kWaves) {
+    for (int e = threadIdx.x; e < nr * Dp; e += 64 * W) {
         const int col = e / Dp, d = e - col * Dp;
-        const float M = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
-        const float o = s_o[col * OP + d] + s_o[(nr + col) * OP + d];
-        float L = 0.0f;
+        const float M = s_M[col], L = s_L[col];
+        float o = 0.0f;
 #pragma unroll
-        for (int ww = 0; ww < kWaves; ++ww) {
-            const float lw = s_l[ww][col];
-            L += s_m[ww][col] == -INFINITY ? (lw != lw ? lw : 0.0f) : fast_exp2(s_m[ww][col] - M) * lw;
-        }
+        for (int h = 0; h < W / 2; ++h) o += s_o[(h * nr + col) * OP + d];
         const int64_t row = row0 + col;
         if (a.nsplit == 1) {
             if (d < a.D) ((QT *)a.o)[row * a.D + d] = (QT)(L == 0.0f ? 0.0f : o / L);
@@ -531,20 +540,22 @@ __global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_kv_blocks_k
         s_last = __hip_atomic_fetch_add(&a.counters[x], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.nsplit - 1;
     __syncthreads();
     if (!s_last) return;
-    merge_splits<QT, NI>(a, row0, nr, s_o);
+    merge_splits<QT, NI, W>(a, row0, nr, s_o);
     if (threadIdx.x == 0) __hip_atomic_store(&a.counters[x], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The kernel for head sizes padded to Dp.
+// The kernel for head sizes padded to Dp and workgroups of 4 or (Dp up to 128) 8 wavefronts.
 template <typename QT>
-inline const void *attn_kernel(int Dp, bool e4m3) {
-#define GT_K(NI) (e4m3 ? (const void *)attn_kv_blocks_kernel<QT, NI, true> : (const void *)attn_kv_blocks_kernel<QT, NI, false>)
-    return Dp == 64 ? GT_K(1) : Dp == 128 ? GT_K(2) : GT_K(4);
+inline const void *attn_kernel(int Dp, bool e4m3, int waves) {
+#define GT_K(NI, W) (e4m3 ? (const void *)attn_kv_blocks_kernel<QT, NI, true, W> : (const void *)attn_kv_blocks_kernel<QT, NI, false, W>)
+    if (Dp == 256) return GT_K(4, 4);
+    if (waves == 8) return Dp == 64 ? GT_K(1, 8) : GT_K(2, 8);
+    return Dp == 64 ? GT_K(1, 4) : GT_K(2, 4);
 #undef GT_K
 }
 
-const void *attn_kernel_f16(int Dp, bool e4m3);
-const void *attn_kernel_bf16(int Dp, bool e4m3);
-const void *attn_kernel_f32(int Dp, bool e4m3);
+const void *attn_kernel_f16(int Dp, bool e4m3, int waves);
+const void *attn_kernel_bf16(int Dp, bool e4m3, int waves);
+const void *attn_kernel_f32(int Dp, bool e4m3, int waves);
 
 }  // namespace gtkvb

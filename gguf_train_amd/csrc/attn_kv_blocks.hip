@@ -9,17 +9,17 @@ namespace {
 
 using namespace gtkvb;
 
-const void *kernel_of(int q_dtype, int Dp, bool e4m3) {
+const void *kernel_of(int q_dtype, int Dp, bool e4m3, int waves) {
     switch (q_dtype) {
-        case GT_F16: return attn_kernel_f16(Dp, e4m3);
-        case GT_BF16: return attn_kernel_bf16(Dp, e4m3);
-        case GT_F32: return attn_kernel_f32(Dp, e4m3);
+        case GT_F16: return attn_kernel_f16(Dp, e4m3, waves);
+        case GT_BF16: return attn_kernel_bf16(Dp, e4m3, waves);
+        case GT_F32: return attn_kernel_f32(Dp, e4m3, waves);
         default: return nullptr;
     }
 }
 
 // Workgroups of `kernel` the device runs at once.
-int64_t resident_groups(const void *kernel) {
+int64_t resident_groups(const void *kernel, int waves) {
     static std::mutex mu;
     static std::map<std::pair<int, const void *>, int64_t> known;
     int dev = 0;
@@ -29,7 +29,7 @@ int64_t resident_groups(const void *kernel) {
     if (it != known.end()) return it->second;
     int cus = 0, per = 0;
     if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * kWaves, 0) != hipSuccess || per <= 0) per = 1;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * waves, 0) != hipSuccess || per <= 0) per = 1;
     return known[{dev, kernel}] = (int64_t)cus * per;
 }
 
@@ -78,15 +78,29 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
     a.shift = c.N == 32 ? 5 : c.N == 64 ? 6 : 7;
     a.units = c.units;
     const int64_t rows = r.H / c.Hkv * r.L, groups = (rows + kColumns - 1) / kColumns;
-    const void *kernel = kernel_of(r.q_dtype, c.Dp, c.e4m3);
-    if (!kernel) return hipErrorInvalidValue;
+    // splits: a workgroup's wavefronts take a unit each per step
+    const int64_t units = (r.max_len / c.N * c.N + kUnit - 1) / kUnit;
     const int64_t grid = c.B * c.Hkv * groups;
     if (grid > 0x7fffffff) return hipErrorInvalidConfiguration;
-    // splits: a workgroup's four wavefronts take a unit each per step
-    const int64_t units = (r.max_len / c.N * c.N + kUnit - 1) / kUnit, steps = std::max<int64_t>(1, (units + kWaves - 1) / kWaves);
-    int n = decode_split_count(grid, steps, resident_groups(kernel), std::min<int64_t>(64, steps));
-    int64_t per = (steps + n - 1) / n;
-    n = (int)((steps + per - 1) / per);
+    const void *kernel = nullptr;
+    int64_t per = 0;
+    int n = 0;
+    auto split = [&](int waves) {
+        kernel = kernel_of(r.q_dtype, c.Dp, c.e4m3, waves);
+        if (!kernel) return;
+        const int64_t steps = std::max<int64_t>(1, (units + waves - 1) / waves);
+        n = decode_split_count(grid, steps, resident_groups(kernel, waves), std::min<int64_t>(64, steps));
+        per = (steps + n - 1) / n;
+        n = (int)((steps + per - 1) / per);
+    };
+    // Workgroups of four wavefronts where they need no splits; otherwise of eight, which leave half the partials to
+    // join or none.  (int8, float16, D128 Hkv8 G4, us with four and eight: B4 S4096 32 tokens 31.5, 27.0; B4 S1024
+    // 32 tokens 16.4, 11.8; B8 S4096 5 tokens 25.9, 21.9; B4 S16384 one token 29.1, 25.9; B1 S4096 one token 10.6,
+    // 11.3; without splits B64 S512 one token 13.8, 20.4; B8 S777 32 tokens 17.8, 24.3.)
+    int waves = 4;
+    split(waves);
+    if (n > 1 && c.Dp <= 128) split(waves = 8);
+    if (!kernel) return hipErrorInvalidValue;
     gt_decode_ws ws{};
     if (n > 1) {
         const size_t out_rows = (size_t)(c.B * r.H * r.L) * (size_t)n;
@@ -96,15 +110,15 @@ hipError_t gt_launch_kv_blocks_attn(const gt_kv_blocks &c, const gt_kv_blocks_at
             a.part_ml = a.part_o + out_rows * (size_t)c.Dp;
         } else {
             n = 1;  // (no workspace for this stream, or a batch that fills the GPU without splits)
-            per = steps;
+            per = (units + waves - 1) / waves;
         }
     }
     a.nsplit = n;
-    a.span = (int)(per * kWaves);
+    a.span = (int)(per * waves);
     note = std::string("decode ") + (c.e4m3 ? "e4m3" : "int8") + " blocks of " + std::to_string(c.N) + " D=" + std::to_string(c.D) +
            " rows=" + std::to_string(rows) + " splits=" + std::to_string(n) +
            " units=" + std::to_string(grid);
     void *args[] = {(void *)&a};
-    const size_t lds = (size_t)attn_lds_floats((int)std::min<int64_t>(rows, kColumns), c.Dp, n) * sizeof(float);
-    return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3(64 * kWaves), args, lds, s);
+    const size_t lds = (size_t)attn_lds_floats((int)std::min<int64_t>(rows, kColumns), c.Dp, n, waves) * sizeof(float);
+    return hipLaunchKernel(kernel, dim3((unsigned)grid, (unsigned)n), dim3((unsigned)(64 * waves)), args, lds, s);
 }
