@@ -8,6 +8,10 @@
 // the end a sum over the 16 lanes of a key's row.  One writer per sum, so no atomics and the same bits each time;
 // where few wavefronts meet many rows the columns are split, and a second launch adds the splits in order.
 //
+// Measured (B4 H32/8 D128 S4096): a float16 cache, one row 9.8 us (3.4 TB/s of keys), int8 and 32 rows of a head 15.7:
+// latency, some 8 us before the first column (length, keys, queries, one after the other) and 1 us a column; with
+// each tile's products in a branch of its own and a tail's lo operands in registers for every wavefront it was 17.6.
+//
 // Operands as attn_kv_blocks.h has them: codes are exact in float16; other rows of keys (bfloat16, float32,
 // Q8_0 values, a block cache's tail) are divided by their own power of two and enter as float16 hi, or as
 // hi + lo where they hold more bits than float16 (float32, Q8_0); float32 queries as hi + lo.
@@ -127,23 +131,27 @@ __device__ inline float key_operands(const KeyDims<KIND> *raw, int D, int g, hal
     return odd ? NAN : pow2(e2);
 }
 
-// grid: (wavefronts' keys / 4, B * Hkv, column splits)
+// grid: (wavefronts' keys / 4, B * Hkv, column splits).  (Two wavefronts a SIMD: without that bound the products' results
+// go through accumulation registers, and a float32 cache's kernel takes more than half of a SIMD's registers.)
 template <typename QT, int SRC, int NI, int TW>
-__global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
+__global__ __launch_bounds__(64 * kWaves, NI <= 2 ? 2 : 1) void attn_key_weights_kernel(Args a) {
     constexpr bool CODES = SRC == kInt8 || SRC == kE4m3;
-    constexpr bool KLO = CODES || SRC == kF32 || SRC == kQ8 || SRC == kAny;  // keys may need lo operands (a tail's do)
+    constexpr bool KLO = SRC == kF32 || SRC == kQ8 || SRC == kAny;  // keys of more bits than float16
     constexpr bool QLO = __is_same(QT, float);
     constexpr int Dp = 64 * NI;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t bg = blockIdx.y, b = bg / a.Hkv, kvh = bg - b * a.Hkv;
     const int len = a.len[b], full = CODES ? len >> a.shift << a.shift : 0;
-    const int k0 = ((int)blockIdx.x * kWaves + w) * 16 * TW;
+    // (the last keys first: the workgroups with fewer keys than the others)
+    const int k0 = ((int)(gridDim.x - 1 - blockIdx.x) * kWaves + w) * 16 * TW;
     if (k0 >= len) return;
 
-    half8 kh[TW][NI][2], kl[TW][NI][2];
+    // the keys' operands; the lo ones of a block cache, which only its tail has, wait in LDS (a lane's own)
+    half8 kh[TW][NI][2], kl[CODES ? 1 : TW][NI][2];
+    __shared__ half8 s_lo[CODES ? kWaves : 1][CODES ? TW : 1][NI][2][64];
     float ksc[TW][4];
-    bool lo_used = !CODES && KLO;
+    const bool tail = CODES && k0 + 16 * TW > full;
     KeyDims<CODES ? kF32 : SRC> raw[CODES ? 1 : TW][NI];
     if constexpr (!CODES) {
 #pragma unroll
@@ -163,14 +171,13 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     kh[kb][i][j] = decode8<SRC == kE4m3>(r[2 * j], r[2 * j + 1]);
-                    kl[kb][i][j] = half8{0, 0, 0, 0, 0, 0, 0, 0};
+                    if (tail) s_lo[w][kb][i][j][lane] = half8{0, 0, 0, 0, 0, 0, 0, 0};
                 }
             }
             const float s = a.ks[bg * (a.units * kUnit >> a.shift) + (t0 >> a.shift)];
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = s;
         } else if constexpr (CODES) {
-            lo_used = true;
             const int room = max(1 << a.shift, kUnit), at = min(t0 - full, room - 16);  // (the last tiles may hold no token)
             const _Float16 *p = a.kt + (bg * 2 * room + at) * Dp + 16 * lane;
 #pragma unroll
@@ -178,13 +185,13 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     kh[kb][i][j] = *(const half8 *)(p + 1024 * i + 8 * j);
-                    kl[kb][i][j] = *(const half8 *)(p + (int64_t)room * Dp + 1024 * i + 8 * j);
+                    s_lo[w][kb][i][j][lane] = *(const half8 *)(p + (int64_t)room * Dp + 1024 * i + 8 * j);
                 }
             const f32x4 s = *(const f32x4 *)(a.kts + bg * room + at + 4 * g);
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = s[i];
         } else {
-            const float s = key_operands<SRC, NI>(raw[kb], a.D, g, kh[kb], kl[kb]);
+            const float s = key_operands<SRC, NI>(raw[kb], a.D, g, kh[kb], kl[CODES ? 0 : kb]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) ksc[kb][i] = __shfl(s, 4 * g + i, 64);
         }
@@ -197,34 +204,68 @@ __global__ __launch_bounds__(64 * kWaves) void attn_key_weights_kernel(Args a) {
         for (int i = 0; i < 4; ++i) sum[kb][i] = 0.0f;
     const int G = a.H / a.Hkv, rows = G * a.L;
     const int c0 = blockIdx.z * a.span, c1 = min(c0 + a.span, a.col_tiles);
-    for (int ct = c0; ct < c1; ++ct) {
-        const int rr = 16 * ct + n, r = min(rr, rows - 1), hh = r / a.L, l = r - hh * a.L;
-        const int lim = rr < rows ? (a.causal ? len - a.L + l + 1 : len) : 0;
-        if (__builtin_amdgcn_ballot_w64(lim > k0) == 0) continue;
-        half8 qh[NI][2], ql[NI][2];
-        const QT *row = (const QT *)a.q + b * a.q_sb + (kvh * G + hh) * a.q_sh + l * a.q_sl;
-        QueryRow<QT, NI> q;
+    // a column's query and log-sum-exp, on their way while the column before is worked on
+    QueryRow<QT, NI> q;
+    const QT *row;
+    int lim;
+    float lse;
+    int hh = (16 * c0 + n) / a.L, l = 16 * c0 + n - hh * a.L;  // the next column's head and token
+    const int heads16 = 16 / a.L, tokens16 = 16 - heads16 * a.L;
+    auto load = [&]() {
+        const int h = min(hh, G - 1);  // (past the last row: some row, which sees no key)
+        lim = hh < G ? (a.causal ? len - a.L + l + 1 : len) : 0;
+        row = (const QT *)a.q + b * a.q_sb + (kvh * G + h) * a.q_sh + l * a.q_sl;
         q.load(row, a.D, a.q_vec, g);
-        const float ls = a.lse[(b * a.H + kvh * G) * a.L + r] * kLog2e;
-        const float f = query_operands<QT, NI>(q, row, a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e;
+        lse = a.lse[(b * a.H + kvh * G + h) * a.L + l];
+        l += tokens16;
+        hh += heads16;
+        if (l >= a.L) l -= a.L, ++hh;
+    };
+    if (c0 < c1) load();
+    for (int ct = c0; ct < c1; ++ct) {
+        half8 qh[NI][2], ql[NI][2];
+        const float f = query_operands<QT, NI>(q, row, a.D, a.q_vec, g, qh, ql) * a.scale * kLog2e, ls = lse * kLog2e;
+        const int seen = lim;
+        if (ct + 1 < c1) load();
+        if (__builtin_amdgcn_ballot_w64(seen > k0) == 0) continue;
+        const bool all = __builtin_amdgcn_ballot_w64(seen >= k0 + 16 * TW) == ~0ull;
+        // the tiles' products side by side: each tile's own follow one another
+        f32x4 c[TW];
 #pragma unroll
-        for (int kb = 0; kb < TW; ++kb) {
-            f32x4 c = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int kb = 0; kb < TW; ++kb) c[kb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto products = [&](auto with_lo) {
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    if constexpr (QLO) c = mma(kh[kb][i][j], ql[i][j], c);
-                    if constexpr (KLO) {
-                        if (lo_used) c = mma(kl[kb][i][j], qh[i][j], c);
-                    }
-                    c = mma(kh[kb][i][j], qh[i][j], c);
-                }
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = fast_exp2(fmaf(c[i], f * ksc[kb][i], -ls));
-                sum[kb][i] += k0 + 16 * kb + 4 * g + i < lim ? p : 0.0f;
-            }
+                    for (int kb = 0; kb < TW; ++kb) {
+                        if constexpr (QLO) c[kb] = mma(kh[kb][i][j], ql[i][j], c[kb]);
+                        if constexpr (decltype(with_lo)::value) c[kb] = mma(s_lo[w][kb][i][j][lane], qh[i][j], c[kb]);
+                        if constexpr (KLO) c[kb] = mma(kl[kb][i][j], qh[i][j], c[kb]);
+                        c[kb] = mma(kh[kb][i][j], qh[i][j], c[kb]);
+                    }
+        };
+        if constexpr (CODES) {
+            if (tail) products(std::true_type{});
+            else products(std::false_type{});
+        } else {
+            products(std::false_type{});
+        }
+#pragma unroll
+        for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[kb][i] = fast_exp2(fmaf(c[kb][i], f * ksc[kb][i], -ls));
+        if (all) {
+#pragma unroll
+            for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[kb][i] += c[kb][i];
+        } else {
+#pragma unroll
+            for (int kb = 0; kb < TW; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[kb][i] += k0 + 16 * kb + 4 * g + i < seen ? c[kb][i] : 0.0f;
         }
     }
 #pragma unroll
@@ -320,7 +361,9 @@ hipError_t gt_launch_key_weights(const gt_key_weights &r, int dev, hipStream_t s
                                                 : kernel_src<float>(src, Dp);
     const int64_t rows = r.H / r.Hkv * r.L, tiles = (rows + 15) / 16, wgs = (r.max_len + keys - 1) / keys;
     // column splits: towards 512 workgroups (two a CU), of 8 columns of 16 rows at least (a wavefront's keys cost
-    // about as much as four)
+    // about as much as four).  A float16 cache, D128 H32/8, us with the attention, without splits and with: B1 S512
+    // L512 110, 32; B1 S2048 L512 150, 72; B1 S4096 L256 136, 106.  Towards 256 workgroups 33, 79, 113, towards 1024
+    // 32, 81, 114; splits of 4 columns 34, 72, 106, of 16 37, 72, 106.
     int64_t splits = std::min<int64_t>(tiles / 8, 512 / std::max<int64_t>(1, wgs * r.B * r.Hkv));
     splits = std::max<int64_t>(1, splits);
     a.col_tiles = (int)tiles;

@@ -26,6 +26,11 @@
 // by its own power of two, as float16 hi + lo, which carry 22 bits.  A token with an infinity or NaN has operands
 // of zero and a NaN for a scale, which only the rows that see it meet.  (Formed here, from the float32 tokens, they
 // took 30 us of a decode step, in loads one after the other.)
+//
+// Measured (GPU time, int8, float16 queries, D128): one token, B16 Hkv8 S8192 46 us, 5.8 TB/s of codes, the rate at which
+// memory is read; B4 S4096 13 us, latency (6.5 us from the start to the first unit's results, 3 the joining of
+// splits, 2 the tail); five tokens B8 S4096 21.8 us and 32 tokens B4 S4096 27, the vector ALU: 64 keys take a
+// wavefront some 500 instructions beside 32 matrix instructions, half of them for making float16 of the codes.
 #pragma once
 
 #include "attn_common.h"

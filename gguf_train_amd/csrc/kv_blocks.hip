@@ -3,10 +3,14 @@
 //
 // Append, bound by HBM (the rows once, a byte per value back): a workgroup owns 64 tokens of one sequence and
 // head (128 where a block has as many) and keeps their values in registers between the largest magnitude and
-// the codes, so a row is read once.  A thread's 16 values are 16 dims of a token for K and 4 tokens x 4 dims for
+// the codes, so a row is read once.  A thread's 16 values are 16 dims of a token for K and 16 tokens of a dim for
 // V, what lies together in the codes' order.  An eviction is the same with the old cache's tokens for source.
 // Read, bound by HBM (mostly the values written): a workgroup stages a unit of 64 tokens' codes in LDS, from
 // which each thread gathers 8 dims of a token.
+//
+// Measured (GPU time, B4 Hkv8 D128, float16, int8): append of 4096 tokens 21 us, 4.8 TB/s (38 before all of a thread's
+// loads were issued together); eviction of 4096 to 2048 tokens 22, of which half the memory rate: V's codes come in
+// single bytes; read of 1500 tokens 13.5, 2.7 TB/s; append of one token 4.5, latency.
 
 #include "gt_internal.h"
 #include "kv_blocks.h"

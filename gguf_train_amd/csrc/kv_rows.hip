@@ -7,10 +7,13 @@
 // gives those that stay their places in order, from ballots and a scan of their counts.  Up to kSelectCached tokens
 // a thread keeps its weights in registers and one scan serves them all, more are read again from the caches, 1024
 // tokens a scan.  Bound: latency, the passes' barriers and counting (LDS atomics), not the 4 bytes a token.  Integer
-// counts alone decide, so the result does not depend on timing.
+// counts alone decide, so the result does not depend on timing.  B4 Hkv8, half of 4096 tokens: 11.4 us (12.7 with a
+// scan for every 1024 tokens); an append of 8192 tokens and an eviction of half 75.0 us against 84.6 with the weights
+// read again in each pass.
 //
 // Moving, HBM-bound: the rows that change place go to scratch memory and from there to their new places, two
-// launches; writing them in place would have workgroups overwrite rows that others have yet to read.
+// launches; writing them in place would have workgroups overwrite rows that others have yet to read.  (16 threads a
+// row, 16 bytes each where the rows are aligned.)
 
 #include "gt_internal.h"
 
