@@ -309,9 +309,10 @@ __device__ inline void append_blocks(const Source &src, const Side &to, int shif
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (!fills(t + 32 * h)) {
-                    // the unit's other block, of tokens to come: the attention reads it, with weights of 0, so it must not
-                    // be e4m3 NaNs
-                    if (h == 1 && t + 32 >= total >> shift << shift) o[1] = make_uint2(0u, 0u);
+                    // the other block, of tokens to come, of a unit whose first is whole: the attention reads it, with
+                    // weights of 0, so it must not be e4m3 NaNs
+                    const int whole = total >> shift << shift;
+                    if (h == 1 && t < whole && t + 32 >= whole) o[1] = make_uint2(0u, 0u);
                     continue;
                 }
                 const float f = inv_of(t + 32 * h);
@@ -408,8 +409,9 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a
     const Side to = slice<DP>(a.to[z], a, bg);
     const RowSource<T, VEC> src = {(const T *)a.src[z] + b * a.st[z][0] + g * a.st[z][1], a.st[z][2], a.st[z][3], to.tail,
                                    held, a.T, a.shift, a.D};
-    // (a decode step that fills no block has none to look at)
-    if (held >> a.shift != total >> a.shift) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, held, total);
+    // (a decode step that fills no block has none to look at, nor has a workgroup past the whole blocks: the grid is of
+    // the sequence that takes most, and another may be at the end of its room)
+    if (held >> a.shift != total >> a.shift && t0 < total >> a.shift << a.shift) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, held, total);
     // The new tail: by the workgroup of its tokens, or, where there is an old one, by the one that has read it.
     const int from = max(held, total >> a.shift << a.shift), old = held & ((1 << a.shift) - 1);
     if (from == total || (int)blockIdx.x != (old ? 0 : from / NT - held / NT)) return;
@@ -435,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_evict_kernel(AppendArgs a)
     const int whole = total >> a.shift << a.shift;
     const bool last = total - t0 <= NT;  // the tail's tokens are among the last workgroup's, or there are none
     const KeptSource<E4M3> src = {from.codes, from.scales, from.tail, s_kept, t0, NT, full, a.shift, a.D, DP, z, late};
-    append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
+    if (t0 < whole) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, 0, total);
     if (last) append_tail<DP>(src, to, a.shift, a.D, z, whole, total, true);
 }
 

@@ -189,6 +189,24 @@ def test_attention_from_the_codes(dev, kind, dtype, B, H, Hkv, L, T, D, block):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("block", [32, 64, 128])
+def test_an_append_to_the_end_of_the_room_leaves_its_neighbours_alone(dev, kind, block):
+    """The grid is of the sequence that takes most blocks; the others are full before its last workgroup."""
+    B, Hkv, D = 3, 2, 64
+    c = g.KVCache(B, Hkv, 256, D, kind, dev, block_tokens=block)
+    parts = [[randn((B, Hkv, n, D), 80 + n + i, torch.float16) for i in range(2)] for n in (99, 32, 125)]
+    for i, (k, v) in enumerate(parts):
+        c.append(k.to(dev), v.to(dev))
+        if i == 0:
+            c.clear(0)
+    assert c.lengths == [157, 256, 256]
+    for got, i in zip(c.read(), range(2)):
+        whole, late = torch.cat([p[i] for p in parts], 2), torch.cat([p[i] for p in parts[1:]], 2)
+        assert torch.equal(got[0, :, :157].double().cpu(), ref.held(late[0], kind, block))
+        assert torch.equal(got[1:].double().cpu(), ref.held(whole[1:], kind, block))
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_ragged_sequences(dev, kind, dtype):
     B, H, Hkv, D = 3, 8, 2, 128
