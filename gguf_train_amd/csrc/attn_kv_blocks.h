@@ -23,7 +23,8 @@
 // bfloat16 results take p' rounded to float16 (2^-12 of each term), float32 results take hi + lo.
 //
 // The tail is one or two more units, of the operands that the append has left: a token's row (K and V) divided
-// by its own power of two, as float16 hi + lo, which carry 22 bits.  A token with an infinity or NaN has operands
+// by its own power of two, as float16 hi + lo, which carry 22 bits (elements below 2^-14 of the row's largest: what
+// is left of 2^-25 of it).  A token with an infinity or NaN has operands
 // of zero and a NaN for a scale, which only the rows that see it meet.  (Formed here, from the float32 tokens, they
 // took 30 us of a decode step, in loads one after the other.)
 //

@@ -412,7 +412,8 @@ __global__ __launch_bounds__(kThreads) void kv_blocks_append_kernel(AppendArgs a
     // (a decode step that fills no block has none to look at, nor has a workgroup past the whole blocks: the grid is of
     // the sequence that takes most, and another may be at the end of its room)
     if (held >> a.shift != total >> a.shift && t0 < total >> a.shift << a.shift) append_blocks<E4M3, DP, NT>(src, to, a.shift, a.D, z, t0, held, total);
-    // The new tail: by the workgroup of its tokens, or, where there is an old one, by the one that has read it.
+    // The new tail: by the workgroup of its tokens, which often has no whole block, or, where there is an old one, by the
+    // one that has read it.  (A workgroup for it alone: B4 Hkv8 D128, 2048 tokens 13.8 against 12.0 us, 2001 14.0, 14.9.)
     const int from = max(held, total >> a.shift << a.shift), old = held & ((1 << a.shift) - 1);
     if (from == total || (int)blockIdx.x != (old ? 0 : from / NT - held / NT)) return;
     __syncthreads();
